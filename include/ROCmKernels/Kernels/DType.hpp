@@ -16,7 +16,11 @@
 #include <rocmkernels_attention.h>
 
 namespace ROCmKernels::Kernels {
-    enum class DType : unsigned char { Float32 = ROCMKERNELS_DTYPE_FLOAT32, Float16 = ROCMKERNELS_DTYPE_FLOAT16 };
+    enum class DType : unsigned char {
+        Float32 = ROCMKERNELS_DTYPE_FLOAT32,
+        Float16 = ROCMKERNELS_DTYPE_FLOAT16,
+        BFloat16 = ROCMKERNELS_DTYPE_BFLOAT16 // no reference counterpart: the paged cache's wrappers only (Cache/KeyValueCache.hpp)
+    };
 
     // DTypeOf<T>::value names the storage type T; only float and __half are defined.
     template<typename T> struct DTypeOf;

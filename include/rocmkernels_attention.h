@@ -195,6 +195,7 @@ ROCMKERNELS_EXPORT int attention64_fp32_backward_ex(const float *q, const float 
 typedef unsigned char rocmkernels_dtype;
 #define ROCMKERNELS_DTYPE_FLOAT32 0
 #define ROCMKERNELS_DTYPE_FLOAT16 1
+#define ROCMKERNELS_DTYPE_BFLOAT16 2 /* the entry points of rocmkernels_cache.h only */
 
 /* Replaces attention_generic_forward (reference Generic/AttentionGeneric.hpp:10-13,
  * Generic/Attention/AttentionGeneric.hip:291-309): windowed forward for headWidth 16, 32 or 64 with q, k, v and

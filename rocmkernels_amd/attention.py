@@ -21,6 +21,7 @@ FUSED_BACKWARD = 2
 DETERMINISTIC = 4
 DTYPE_FLOAT32 = 0  # rocmkernels_dtype / ROCmKernels::Kernels::DType::Float32
 DTYPE_FLOAT16 = 1
+DTYPE_BFLOAT16 = 2  # the cache entry points only
 HIP_ERROR_INVALID_VALUE = 1
 
 
@@ -28,6 +29,18 @@ class Strides(ctypes.Structure):
     """Element strides of a [batch][head][token] tensor (C struct rocmkernels_strides)."""
 
     _fields_ = [("batch", I), ("head", I), ("token", I)]
+
+
+class Cache(ctypes.Structure):
+    """A paged 8-bit key/value cache (C struct rocmkernels_cache)."""
+
+    _fields_ = [("keys", P), ("values", P), ("scales", P), ("pages", I), ("page_size", I), ("heads", I), ("width", I)]
+
+
+class Sequences(ctypes.Structure):
+    """Packed sequences and their pages (C struct rocmkernels_sequences)."""
+
+    _fields_ = [("starts", P), ("lengths", P), ("table", P), ("batch", I), ("tokens", I), ("columns", I), ("table_stride", I)]
 
 
 S = Strides
@@ -56,6 +69,9 @@ ENTRY_POINTS = {
     "attention64_fp32_backward_ex": _BACKWARD_CODE,
     "attention_generic_forward": [P, P, P, P, P, P, I, I, I, I, I, I, S, S, S, S, ctypes.c_ubyte, P],
     "rotary_fp32": [P, P, P, P, P, P, I, I, I, I, S, S, S, S, P],
+    "attention_cache_append": [P, P, P, P, P, P, Cache, Sequences, I, I, S, S, S, S, S, S, ctypes.c_ubyte, P],
+    "attention_cache_forward": [P, Cache, Sequences, P, P, I, I, I, I, S, S, ctypes.c_ubyte, P, ctypes.c_size_t, P],
+    "attention_cache_workspace": [Cache, Sequences, I, I, ctypes.c_ubyte, ctypes.POINTER(ctypes.c_size_t)],
 }
 
 _lib = None

@@ -1,0 +1,82 @@
+// How a cache call is cut into workgroups: host and device arithmetic without any HIP call (tests/cpp/cache_plan_check.cpp runs it on
+// the CPU).
+//
+// starts, the division of the packed rows over sequences, is device memory, so the host sizes a launch from tokens and batch
+// alone: sequence b owns the units from floor((starts[b] * mul + b * add) / div) up to the next sequence's first. For tiles of `rows`
+// flattened rows (mul = heads of a group, add = rows - 1, div = rows) these are at least ceil(n / rows) units for n rows, and
+// exactly one for each sequence of a decoding batch; for pages of `size` tokens (mul = 1, add = 2 size - 2, div = size) at least
+// floor((n + 2 size - 2) / size), the most pages that n rows touch.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace rk {
+
+constexpr int kBlockTokens = 16;   // tokens of one block of a page: K rows [16][D], V columns [D][16]
+constexpr int kMaxPage = 128;
+constexpr int kMaxRows = 256;      // no tile of the attention kernels has more rows
+constexpr int kStep = 64;          // keys of a step of the attention kernels
+
+struct SequenceView {
+    const int *starts, *lengths, *table;
+    int batch, tokens, columns, table_stride;
+};
+
+__host__ __device__ inline uint32_t unit_base(const int start, const int b, const uint32_t mul, const uint32_t add, const uint32_t div) {
+    return (static_cast<uint32_t>(start) * mul + static_cast<uint32_t>(b) * add) / div;
+}
+
+// Whether sequence b's first unit is not past `unit`: floor(x / div) <= unit exactly where x < (unit + 1) * div.
+__host__ __device__ inline bool reaches(const int start, const int b, const uint32_t unit, const uint32_t mul, const uint32_t add,
+        const uint32_t div) {
+    return static_cast<uint32_t>(start) * mul + static_cast<uint32_t>(b) * add < (unit + 1) * div;
+}
+
+// The search's rounds: 64 lanes test sequences `search_step` apart.
+__host__ __device__ inline int search_step(const int span) { return (span + 63) / 64; }
+
+inline long long row_units(const long long flat_rows, const int batch, const int rows) {
+    return (flat_rows + static_cast<long long>(batch) * (rows - 1)) / rows;
+}
+
+inline long long page_units(const int tokens, const int batch, const int size) {
+    return (tokens + static_cast<long long>(batch) * (2 * size - 2)) / size;
+}
+
+// Rows of a sequence are flattened to (row, query head of the group) and cut into tiles of `rows`; the keys a tile sees are cut into
+// chunks of `chunk_steps` steps, `chunks` at most.
+struct ForwardPlan {
+    int rows, units, chunk_steps, chunks;
+    size_t workspace;      // bytes this call needs
+    size_t workspace_most; // and with any smaller window
+};
+
+inline ForwardPlan plan_cache_forward(const int width, const int dtype, const SequenceView &s, const int heads, const int query_heads,
+        const int max_keys, const int radius) {
+    (void)dtype;
+    ForwardPlan p;
+    const int group = query_heads / heads;
+    const long long flat = static_cast<long long>(s.tokens) * group;
+    p.rows = flat <= 16ll * s.batch ? 16 : 32;
+    p.units = static_cast<int>(row_units(flat, s.batch, p.rows));
+    // The keys that a tile may see: all, or its window.
+    long long span = max_keys;
+    if (radius >= 0) span = std::min(span, 2ll * radius + 1 + (p.rows + group - 1) / group + kStep);
+    const long long steps = (span + kStep - 1) / kStep;
+    const long long pairs = static_cast<long long>(p.units) * heads;
+    const long long wanted = (2048 + pairs - 1) / std::max(pairs, 1ll);
+    const long long chunks = std::min(wanted, std::max(1ll, steps / 8)); // grows with the keys and the window
+    p.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks);
+    p.chunks = static_cast<int>((steps + p.chunk_steps - 1) / p.chunk_steps);
+    const size_t chunk_bytes = static_cast<size_t>(pairs) * p.rows * (width + 4) * sizeof(float);
+    p.workspace = p.chunks > 1 ? chunk_bytes * p.chunks : 0;
+    p.workspace_most = chunks > 1 ? chunk_bytes * chunks : 0;
+    return p;
+}
+
+} // namespace rk

@@ -1,0 +1,84 @@
+// Host check of the arithmetic that maps workgroups to sequences (cache_plan.hpp): for random divisions of rows over sequences,
+// every tile of rows and every page that receives rows has exactly one unit, units of one sequence never reach into the next
+// one's, and the search finds the sequence of a unit. Random plans stay within their limits, and a smaller window never needs more
+// workspace than the largest.
+#include "cache_plan.hpp"
+
+#include <cstdio>
+#include <random>
+#include <vector>
+
+namespace {
+int failures = 0;
+void check(const bool ok, const char *what) {
+    if (!ok && ++failures < 20) std::printf("FAIL %s\n", what);
+}
+
+// The device's search, one lane after the other.
+int search(const std::vector<int> &starts, const int batch, const int tokens, const uint32_t unit, const uint32_t mul, const uint32_t add,
+        const uint32_t div) {
+    int low = 0, span = batch;
+    while (span > 1) {
+        const int step = rk::search_step(span);
+        int hit = 0;
+        for (int lane = 0; lane < 64; ++lane) {
+            const int b = low + lane * step;
+            if (lane * step < span && rk::reaches(std::min(std::max(starts[b], 0), tokens), b, unit, mul, add, div)) hit = lane;
+        }
+        low += hit * step;
+        span = std::min(step, span - hit * step);
+    }
+    return low;
+}
+} // namespace
+
+int main() {
+    std::mt19937 rng(7);
+    auto pick = [&](const int low, const int high) { return low + static_cast<int>(rng() % (high - low + 1)); };
+    for (int round = 0; round < 4000; ++round) {
+        const int batch = round % 50 == 0 ? pick(1000, 9000) : pick(1, 200), most = pick(0, 3) == 0 ? 400 : 3;
+        std::vector<int> starts(batch + 1, 0);
+        for (int b = 0; b < batch; ++b) starts[b + 1] = starts[b] + (pick(0, 3) == 0 ? 0 : pick(0, most));
+        const int tokens = starts[batch] + pick(0, 2), group = pick(1, 9);
+        // Row tiles.
+        for (const int rows : {16, 32, 128}) {
+            const uint32_t mul = group, add = rows - 1, div = rows;
+            const long long units = rk::row_units(static_cast<long long>(tokens) * group, batch, rows);
+            for (int b = 0; b < batch; ++b) {
+                const uint32_t base = rk::unit_base(starts[b], b, mul, add, div), next = rk::unit_base(starts[b + 1], b + 1, mul, add, div);
+                const uint32_t tiles = (static_cast<uint32_t>(starts[b + 1] - starts[b]) * group + rows - 1) / rows;
+                check(base + tiles <= next && next <= static_cast<uint32_t>(units), "row tiles reach into the next sequence");
+                if (b % 7 == 0 || batch < 300)
+                    for (uint32_t t = 0; t < tiles; t += std::max(1u, tiles / 3))
+                        check(search(starts, batch, tokens, base + t, mul, add, div) == b, "search for a row tile");
+            }
+        }
+        // Pages.
+        const int size = 16 * pick(1, 8);
+        const uint32_t add = 2 * size - 2;
+        const long long units = rk::page_units(tokens, batch, size);
+        for (int b = 0; b < batch; ++b) {
+            const int count = starts[b + 1] - starts[b], first = pick(0, 500);
+            const uint32_t pages = count ? (first + count - 1) / size - first / size + 1 : 0;
+            const uint32_t base = rk::unit_base(starts[b], b, 1, add, size);
+            check(base + pages <= rk::unit_base(starts[b + 1], b + 1, 1, add, size), "pages reach into the next sequence");
+            check(base + pages <= static_cast<uint32_t>(units), "more pages than units");
+            if (pages && (b % 7 == 0 || batch < 300)) check(search(starts, batch, tokens, base + pages - 1, 1, add, size) == b, "search for a page");
+        }
+        // Tokens.
+        for (int b = 0; b < batch; b += 1 + batch / 50)
+            if (starts[b + 1] > starts[b]) check(search(starts, batch, tokens, starts[b + 1] - 1, 1, 0, 1) == b, "search for a token");
+        // Plans.
+        const rk::SequenceView s{nullptr, nullptr, nullptr, batch, tokens, 1, 1};
+        const int heads = pick(1, 12), keys = pick(0, 2) ? pick(1, 5000) : pick(1, 200000), width = 32 << pick(0, 2), dtype = pick(0, 2);
+        const size_t whole = rk::plan_cache_forward(width, dtype, s, heads, heads * group, keys, -1).workspace_most;
+        for (const int radius : {-1, 0, 1, 100, 777, 5000, 100000}) {
+            const rk::ForwardPlan p = rk::plan_cache_forward(width, dtype, s, heads, heads * group, keys, radius);
+            check(p.rows <= rk::kMaxRows && p.chunks >= 1 && p.chunk_steps >= 1, "plan");
+            check(p.workspace <= whole, "a window needs more workspace than the whole");
+            if (radius < 0) check(static_cast<long long>(p.chunks) * p.chunk_steps * 64 >= keys, "chunks do not cover the keys");
+        }
+    }
+    std::printf("%d failure(s)\n", failures);
+    return failures != 0;
+}
