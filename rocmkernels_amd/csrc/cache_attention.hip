@@ -23,6 +23,8 @@
 #include "cache_device.hpp"
 #include "cache_launch.hpp"
 
+#include <algorithm>
+
 namespace rk {
 
 namespace {
@@ -74,19 +76,26 @@ struct Tile {
     int step0, steps, chunks;  // steps of 64 keys that any of them sees, and the chunks they are cut into
 };
 
-__device__ __forceinline__ Tile tile_of(const CacheForwardArgs &a, const ForwardPlan &plan, const uint32_t unit, const int group) {
+__device__ __forceinline__ Tile tile_of(const CacheForwardArgs &a, const ForwardPart &part, const uint32_t unit, const int group) {
     Tile t;
-    t.s = find_sequence(a.seqs, unit, group, plan.rows - 1, plan.rows);
-    const uint32_t index = unit - t.s.base;
+    uint32_t index;
+    if (part.direct) {
+        t.s = sequence_at(a.seqs, static_cast<int>(unit / part.direct));
+        index = unit % part.direct;
+    } else {
+        t.s = find_sequence(a.seqs, unit, group, part.rows - 1, part.rows);
+        index = unit - t.s.base;
+    }
     const uint32_t flat = static_cast<uint32_t>(t.s.count) * group;
-    t.row0 = static_cast<int>(index * plan.rows);
-    t.rows = index < (flat + plan.rows - 1) / plan.rows ? min(plan.rows, static_cast<int>(flat) - t.row0) : 0;
+    const bool taken = flat >= static_cast<uint32_t>(part.least) && flat <= static_cast<uint32_t>(part.most) &&
+            index < (flat + part.rows - 1) / part.rows;
+    t.row0 = taken ? static_cast<int>(index * part.rows) : 0;
+    t.rows = taken ? min(part.rows, static_cast<int>(flat) - t.row0) : 0;
     t.vis = Visibility{min(t.s.length, a.max_keys), a.radius, a.causal};
-    const int first = t.s.first + t.row0 / group, last = t.s.first + (t.row0 + t.rows - 1) / group;
-    const int low = t.vis.low(first), high = t.vis.high(last);
+    const int low = t.vis.low(t.s.first + t.row0 / group), high = t.vis.high(t.s.first + max(t.row0 + t.rows - 1, 0) / group);
     t.step0 = low / kStep;
     t.steps = t.rows > 0 && high > low ? (high + kStep - 1) / kStep - t.step0 : 0;
-    t.chunks = (t.steps + plan.chunk_steps - 1) / plan.chunk_steps;
+    t.chunks = (t.steps + part.chunk_steps - 1) / part.chunk_steps;
     return t;
 }
 
@@ -112,10 +121,10 @@ struct Partial {
     float *acc, *stats;
 };
 template<int D>
-__device__ __forceinline__ Partial partial_of(const CacheForwardArgs &a, const ForwardPlan &plan, const int64_t slot, const int row) {
-    float *const base = static_cast<float *>(a.workspace);
-    const int64_t slots = static_cast<int64_t>(plan.units) * a.cache.heads * plan.chunks, r = slot * plan.rows + row;
-    return {base + r * D, base + slots * plan.rows * D + r * 4};
+__device__ __forceinline__ Partial partial_of(const CacheForwardArgs &a, const ForwardPart &part, const int64_t slot, const int row) {
+    float *const base = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + part.workspace_at);
+    const int64_t slots = static_cast<int64_t>(part.units) * a.cache.heads * part.chunks, r = slot * part.rows + row;
+    return {base + r * D, base + slots * part.rows * D + r * 4};
 }
 
 // The two terms of 8 values that are already scaled into fp16's range.
@@ -131,7 +140,7 @@ __device__ __forceinline__ void split_terms(f16x8 &hi, f16x8 &lo, const float (&
 // NQ tiles of 16 rows a workgroup.
 template<int T, int D, int NQ, bool VEC>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_kernel(const CacheForwardArgs a,
-        const ForwardPlan plan) {
+        const ForwardPart part) {
     constexpr bool TWO = T == kFloat32;
     constexpr int KC = D / 32;                   // MFMAs of a score tile
     constexpr int KL = D >= 64 ? D / 64 : 1;     // loads of a K row tile
@@ -144,15 +153,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     const int lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int heads = a.cache.heads, group = a.query_heads / heads;
-    const uint32_t slot = blockIdx.x, pair = slot / plan.chunks;
-    const int chunk = static_cast<int>(slot - pair * plan.chunks);
+    const uint32_t slot = blockIdx.x, pair = slot / part.chunks;
+    const int chunk = static_cast<int>(slot - pair * part.chunks);
     const uint32_t unit = pair / heads;
     const int head = static_cast<int>(pair - unit * heads);
 
-    const Tile t = tile_of(a, plan, unit, group);
+    const Tile t = tile_of(a, part, unit, group);
     if (t.rows <= 0 || chunk >= max(t.chunks, 1)) return;
-    const int step_begin = t.step0 + chunk * plan.chunk_steps;
-    const int step_end = t.step0 + min(t.steps, (chunk + 1) * plan.chunk_steps);
+    const int step_begin = t.step0 + chunk * part.chunk_steps;
+    const int step_end = t.step0 + min(t.steps, (chunk + 1) * part.chunk_steps);
 
     // This lane's rows: q in operand order, the factor of its scores, and the keys it sees.
     f16x8 qh[NQ][KC], ql[TWO ? NQ : 1][TWO ? KC : 1];
@@ -274,7 +283,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         }
         const int key0 = kStep * step, base = key0 + 16 * g;
         const bool full = key0 >= all_low && key0 + kStep <= all_high && ((absent >> (4 * turn)) & 15u) == 0;
-        uint32_t visible[NQ];
+        uint32_t visible[NQ], held = 0;
         bool any_nan = false;
         if (!full) {
             const bool here = !((absent >> (4 * turn + g)) & 1u);
@@ -287,15 +296,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
                     for (int j = 0; j < 4; ++j) sc[n][i][j] = (visible[n] >> (4 * i + j)) & 1u ? sc[n][i][j] : -INFINITY;
                 }
             }
-            // Bytes behind the sequence's end may hold anything, and 0 times NaN is no 0.
-            const uint32_t held = here ? bit_range(0, t.vis.length - base - 1) & 0xffffu : 0u;
+            // Bytes behind the sequence's end may hold anything, and 0 times NaN is no 0: NaN counts for the rows that see its key.
+            held = here ? bit_range(0, t.vis.length - base - 1) & 0xffffu : 0u;
             uint32_t nans = 0;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x.v[d][i] &= byte_mask(held >> (4 * i));
-                    nans |= nan_bytes(x.v[d][i]);
+                    const uint32_t w = x.v[d][i] & byte_mask(held >> (4 * i)), bad = nan_bytes(w);
+                    x.v[d][i] = w & ~bad;
+                    nans |= bad;
                 }
             }
             any_nan = __ballot(nans != 0) != 0;
@@ -340,32 +350,42 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             for (int d = 0; d < DT; ++d) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    u32x2 bytes{x.v[d][2 * u], x.v[d][2 * u + 1]};
-                    if (any_nan) {
-                        bytes[0] &= ~nan_bytes(bytes[0]);
-                        bytes[1] &= ~nan_bytes(bytes[1]);
-                    }
-                    const f16x8 v = widen(bytes[0], bytes[1]);
+                    const f16x8 v = widen(x.v[d][2 * u], x.v[d][2 * u + 1]);
                     acc[n][d] = mfma_16(v, wh[u], acc[n][d]);
                     if constexpr (TWO) acc[n][d] = mfma_16(v, wl[u], acc[n][d]);
                 }
             }
-            if (any_nan) {
-                // NaN in V reaches the rows that see its key and no other: count them with a product of ones.
+        }
+        if (__builtin_expect(any_nan, 0)) {
+            // Count the NaN values that each row sees with a product of ones (0x38 is 1.0 in e4m3); V's bytes are read again.
+            const int64_t vb = max(__shfl(place, 4 * turn + g), 0);
+            const uint8_t *const v = a.cache.values + vb * (kBlockTokens * D) + col * 16;
+#pragma unroll 1
+            for (int n = 0; n < NQ; ++n) {
                 f16x8 sees[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sees[u][j] = static_cast<_Float16>((visible[n] >> (8 * u + j)) & 1u ? 1.0f : 0.0f);
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t bits = visible[0];
+                        if constexpr (NQ > 1) bits = n == 0 ? visible[0] : visible[NQ - 1];
+                        sees[u][j] = static_cast<_Float16>((bits >> (8 * u + j)) & 1u ? 1.0f : 0.0f);
+                    }
                 }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
+                    const u32x4 y = *reinterpret_cast<const u32x4 *>(v + d * 256);
                     f32x4 hits{};
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) // 0x38 is 1.0 in e4m3
-                        hits = mfma_16(widen(nan_bytes(x.v[d][2 * u]) & 0x38383838u, nan_bytes(x.v[d][2 * u + 1]) & 0x38383838u), sees[u], hits);
+                    for (int u = 0; u < 2; ++u)
+                        hits = mfma_16(widen(nan_bytes(y[2 * u] & byte_mask(held >> (8 * u))) & 0x38383838u,
+                                               nan_bytes(y[2 * u + 1] & byte_mask(held >> (8 * u + 4))) & 0x38383838u),
+                                sees[u], hits);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[n][d][j] = hits[j] > 0.0f ? NAN : acc[n][d][j];
+                    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                        for (int k = 0; k < NQ; ++k) acc[k][d][j] = k == n && hits[j] > 0.0f ? NAN : acc[k][d][j];
+                    }
                 }
             }
         }
@@ -419,7 +439,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             const int flat = t.row0 + r, token = flat / group;
             finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, o, sum, reference, most, f == 0);
         } else {
-            const Partial p = partial_of<D>(a, plan, slot, r);
+            const Partial p = partial_of<D>(a, part, slot, r);
 #pragma unroll
             for (int j = 0; j < SPAN; j += 4) *reinterpret_cast<f32x4 *>(p.acc + f + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
             if (f == 0) *reinterpret_cast<f32x4 *>(p.stats) = f32x4{reference, sum, most, 0.0f};
@@ -427,57 +447,395 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     }
 }
 
-// Joins the chunks of a tile, in their order.
+// Tiles of 128 rows, 32 a wave, that share the keys: each step's 64 keys are read once, widened to fp16 and staged in LDS for the
+// four waves (double-buffered, one barrier a step), so a byte of the cache is converted once for 128 rows. Products are on
+// v_mfma_f32_32x32x16_f16, S^T = K Q^T and O^T = V^T P^T as above: accumulator register v of a lane in half h holds row 8 (v / 4)
+// + 4 h + v % 4 of a 32-key tile. Row r stands for token 16 (r / 16) + 8 ((r / 4) % 2) + 4 ((r / 8) % 2) + r % 4, so registers 8 u .. 8 u + 7
+// hold the tokens 16 u + 8 h .. + 7: one page's scales for eight scores, and the operand of V's block u as it lies in memory.
+// Staged layouts: K [8-feature chunk][token] and V [block][half][feature] of 16 bytes, so operand reads cover 512 contiguous bytes a
+// half-wave; a K chunk is padded by 16 * 128 / D bytes, which puts the writes of 16 neighbouring lanes on distinct banks.
 template<int T, int D, bool VEC>
-__global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForwardArgs a, const ForwardPlan plan) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_large_kernel(const CacheForwardArgs a,
+        const ForwardPart part) {
+    constexpr bool TWO = T == kFloat32;
+    constexpr int KC = D / 16;                       // MFMAs of a 32-key score tile
+    constexpr int DT = D / 32;                       // output tiles
+    constexpr int K_CHUNK = kStep * 16 + 16 * 128 / D;
+    constexpr int K_BYTES = D / 8 * K_CHUNK, V_BYTES = kStep * D * 2;
+    constexpr int LOADS = (kStep * D / 16 + kThreads - 1) / kThreads; // 16-byte loads of K, and of V, of a thread
+    constexpr bool ALL = kStep * D / 16 >= kThreads; // D = 32: half the threads load
+    __shared__ __align__(16) uint8_t staged[2][K_BYTES + V_BYTES];
+    __shared__ int nan_flags[2][kWaves];
+
+    const int lane = threadIdx.x & (kWave - 1), col = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int heads = a.cache.heads, group = a.query_heads / heads;
-    const uint32_t pair = blockIdx.x, unit = pair / heads;
-    const int head = static_cast<int>(pair - unit * heads);
-    const Tile t = tile_of(a, plan, unit, group);
-    if (t.rows <= 0 || t.chunks <= 1) return;
-    constexpr int SPAN = 8;
-    const int64_t slot = static_cast<int64_t>(pair) * plan.chunks;
-    for (int i = threadIdx.x; i < t.rows * (D / SPAN); i += kThreads) {
-        const int r = i / (D / SPAN), f = i % (D / SPAN) * SPAN;
-        float reference = -INFINITY, most = -INFINITY, sum = 0.0f, o[SPAN] = {};
-        for (int c = 0; c < t.chunks; ++c) {
-            const f32x4 s = *reinterpret_cast<const f32x4 *>(partial_of<D>(a, plan, slot + c, r).stats);
-            reference = fmaxf(reference, s[0]);
-            most = fmaxf(most, s[2]);
+    // Workgroups go round the 8 XCDs: give each XCD whole heads, whose keys then stay in its L2, and of a head the last tiles
+    // (under a causal mask the longest) first.
+    const uint32_t pairs = static_cast<uint32_t>(part.units) * heads, total = pairs * part.chunks;
+    const uint32_t xcd = blockIdx.x % 8, place_in_order = xcd * (total / 8) + min(xcd, total % 8) + blockIdx.x / 8;
+    const int head = static_cast<int>(place_in_order / (part.units * part.chunks));
+    const uint32_t rest = place_in_order - static_cast<uint32_t>(head) * part.units * part.chunks;
+    const uint32_t unit = part.units - 1 - rest / part.chunks;
+    const int chunk = static_cast<int>(rest % part.chunks);
+    const int64_t slot = (static_cast<int64_t>(unit) * heads + head) * part.chunks + chunk;
+
+    const Tile t = tile_of(a, part, unit, group);
+    if (t.rows <= 0 || chunk >= max(t.chunks, 1)) return;
+    const int step_begin = t.step0 + chunk * part.chunk_steps;
+    const int steps = t.step0 + min(t.steps, (chunk + 1) * part.chunk_steps) - step_begin;
+
+    // This wave's rows; a wave past the tile's last row only loads.
+    const int wave_row0 = 32 * wave, wave_rows = min(32, t.rows - wave_row0);
+    const int r = wave_row0 + col;
+    const bool used = r < t.rows;
+    const int flat = t.row0 + (used ? r : 0), i = flat / group, query_head = head * group + (flat - i * group);
+    const int low = t.vis.low(t.s.first + i), high = t.vis.high(t.s.first + i);
+    const int wave_first = t.s.first + (t.row0 + min(wave_row0, t.rows - 1)) / group;
+    const int wave_last = t.s.first + (t.row0 + min(wave_row0 + 31, t.rows - 1)) / group;
+    const int any_low = t.vis.low(wave_first), any_high = t.vis.high(wave_last);  // keys that some row of the wave sees
+    const int all_low = t.vis.low(wave_last), all_high = t.vis.high(wave_first);  // and keys that every one sees
+    const int tile_low = t.vis.low(t.s.first + (t.row0 + t.rows - 1) / group), tile_high = t.vis.high(t.s.first + t.row0 / group);
+
+    f16x8 qh[KC], ql[TWO ? KC : 1];
+    float c2;
+    {
+        const int64_t row = static_cast<int64_t>(t.s.row0 + i) * a.qs.token + static_cast<int64_t>(query_head) * a.qs.head;
+        float x[KC][8];
+#pragma unroll
+        for (int k = 0; k < KC; ++k) load8<T, VEC>(x[k], a.q, row + 16 * k + 8 * h);
+        float scale = 1.0f, back = 1.0f;
+        if constexpr (T != kFloat16) {
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[k][j]));
+            }
+            const int e = clamped(static_cast<int>(__float_as_uint(halves_max(most)) >> 23) - 127, -100, 127);
+            scale = power(14 - e);
+            back = power(e - 14);
         }
-        for (int c = 0; c < t.chunks; ++c) {
-            const Partial p = partial_of<D>(a, plan, slot + c, r);
-            const f32x4 s = *reinterpret_cast<const f32x4 *>(p.stats);
-            const float alpha = s[0] == reference ? 1.0f : exp2_fast(s[0] - reference);
-            sum = fmaf(s[1], alpha, sum);
+        c2 = back * (kLog2e / sqrtf(static_cast<float>(D)));
 #pragma unroll
-            for (int j = 0; j < SPAN; j += 4) {
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(p.acc + f + j);
+        for (int k = 0; k < KC; ++k) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[j + k] = fmaf(x[k], alpha, o[j + k]);
+            for (int j = 0; j < 8; ++j) x[k][j] *= scale;
+            split_terms<TWO>(qh[k], ql[TWO ? k : 0], x[k]);
+        }
+    }
+
+    float M = -INFINITY, l = 0.0f, m = -INFINITY;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+
+    // The 64 blocks of the next 16 steps, one a lane: the block's place in the cache (-1: none) and its exponents, as bytes.
+    const int blocks = a.cache.page_size / kBlockTokens;
+    int place = -1, exponents = 0;
+    auto look_up = [&](const int index) __attribute__((always_inline)) {
+        const int s = index + lane / 4, position = kStep * (step_begin + s) + kBlockTokens * (lane % 4);
+        place = -1;
+        exponents = 0;
+        if (s < steps && position < t.vis.length) {
+            const int column = position / a.cache.page_size;
+            const int page = a.seqs.table[static_cast<int64_t>(t.s.b) * a.seqs.table_stride + column];
+            if (page >= 0 && page < a.cache.pages) {
+                const int cell = page * heads + head;
+                place = cell * blocks + (position - column * a.cache.page_size) / kBlockTokens;
+                exponents = (scale_exponent(a.cache.scales[2 * static_cast<int64_t>(cell)]) & 255) |
+                        ((scale_exponent(a.cache.scales[2 * static_cast<int64_t>(cell) + 1]) & 255) << 8);
             }
         }
-        const int flat = t.row0 + r, token = flat / group;
-        finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, o, sum, reference, most, f == 0);
+    };
+    // A step's bytes on their way to LDS, and the exponents of its four blocks (as bytes, in scalar registers).
+    u32x4 raw_k[LOADS], raw_v[LOADS];
+    struct Scales {
+        int exps[4], places[4];
+        uint32_t absent;
+    };
+    auto load = [&](Scales &e, const int index) __attribute__((always_inline)) {
+        const int turn = index % 16;
+        if (turn == 0) look_up(index);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            e.exps[b] = __builtin_amdgcn_readlane(exponents, 4 * turn + b);
+            e.places[b] = __builtin_amdgcn_readlane(place, 4 * turn + b);
+        }
+        e.absent = static_cast<uint32_t>(__ballot(place < 0) >> (4 * turn)) & 15u;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            // K: token x / (D / 16), 16 of its features; V: block x / D, feature x % D. Blocks that are not there read the cache's first.
+            const int x = threadIdx.x + n * kThreads, token = x / (D / 16), block = x / D;
+            const int64_t kb = max(__shfl(place, 4 * turn + min(token / 16, 3)), 0), vb = max(__shfl(place, 4 * turn + min(block, 3)), 0);
+            if (ALL || x < kStep * D / 16) {
+                raw_k[n] = *reinterpret_cast<const u32x4 *>(a.cache.keys + kb * (kBlockTokens * D) + (token % 16) * D + (x % (D / 16)) * 16);
+                raw_v[n] = *reinterpret_cast<const u32x4 *>(a.cache.values + vb * (kBlockTokens * D) + (x % D) * 16);
+            }
+        }
+    };
+    auto stage = [&](const int index, const uint32_t absent) __attribute__((always_inline)) {
+        uint8_t *const k = staged[index & 1], *const v = k + K_BYTES;
+        const int key0 = kStep * (step_begin + index);
+        const bool full = key0 >= tile_low && key0 + kStep <= tile_high && absent == 0; // no key that any row does not see
+        uint32_t nans = 0;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int x = threadIdx.x + n * kThreads, token = x / (D / 16), block = x / D;
+            if (!ALL && x >= kStep * D / 16) continue;
+            if (!full) {
+                // Bytes behind the sequence's end may hold anything, and 0 times NaN is no 0: NaN counts for the rows that see its key.
+                const uint32_t held = (absent >> block) & 1u ? 0u : bit_range(0, t.vis.length - key0 - 16 * block - 1) & 0xffffu;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = raw_v[n][j] & byte_mask(held >> (4 * j)), bad = nan_bytes(w);
+                    raw_v[n][j] = w & ~bad;
+                    nans |= bad;
+                }
+            }
+            uint8_t *const to = k + (x % (D / 16)) * (2 * K_CHUNK) + token * 16;
+            *reinterpret_cast<f16x8 *>(to) = widen(raw_k[n][0], raw_k[n][1]);
+            *reinterpret_cast<f16x8 *>(to + K_CHUNK) = widen(raw_k[n][2], raw_k[n][3]);
+            uint8_t *const tv = v + (2 * block * D + x % D) * 16;
+            *reinterpret_cast<f16x8 *>(tv) = widen(raw_v[n][0], raw_v[n][1]);
+            *reinterpret_cast<f16x8 *>(tv + D * 16) = widen(raw_v[n][2], raw_v[n][3]);
+        }
+        const bool any = __ballot(nans != 0) != 0;
+        if (lane == 0) nan_flags[index & 1][wave] = any;
+    };
+    // Operand row of this lane: the token that row `col` of a 32-key tile stands for.
+    const int token_of_row = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+
+    auto compute = [&](const int index, const Scales &e) __attribute__((always_inline)) {
+        const int key0 = kStep * (step_begin + index);
+        if (wave_rows <= 0 || key0 >= any_high || key0 + kStep <= any_low) return;
+        const uint8_t *const k = staged[index & 1] + token_of_row * 16 + h * K_CHUNK;
+        const uint8_t *const v = staged[index & 1] + K_BYTES + (h * D + col) * 16;
+        f32x16 sc[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            sc[n] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const f16x8 w = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK) + n * 512);
+                sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[c], sc[n], 0, 0, 0);
+                if constexpr (TWO) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[c], sc[n], 0, 0, 0);
+            }
+        }
+        const bool full = key0 >= all_low && key0 + kStep <= all_high && e.absent == 0;
+        bool any_nan = false;
+        if (!full) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int base = key0 + 16 * b + 8 * h;
+                const uint32_t visible = (e.absent >> b) & 1u ? 0u : bit_range(low - base, high - base - 1);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sc[b / 2][8 * (b % 2) + j] = (visible >> j) & 1u ? sc[b / 2][8 * (b % 2) + j] : -INFINITY;
+            }
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) any_nan |= nan_flags[index & 1][w] != 0;
+        }
+        float c[4], candidate = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            c[b] = fmaxf(c2 * power(static_cast<int8_t>(e.exps[b])), 1.17549435e-38f); // > 0, so that hidden scores stay -inf
+            float most = sc[b / 2][8 * (b % 2)];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[b / 2][8 * (b % 2) + j]);
+            most *= c[b];
+            m = fmaxf(m, most);
+            candidate = fmaxf(candidate, most + static_cast<float>(static_cast<int8_t>(e.exps[b] >> 8)));
+        }
+        if (__ballot(candidate > M + kLazyRange)) {
+            const float raised = halves_max(fmaxf(M, candidate));
+            const float alpha = M == raised ? 1.0f : exp2_fast(M - raised);
+            M = raised;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= alpha;
+        }
+        const float reference = (M == -INFINITY ? 0.0f : M) - kWeightShift;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int ev = static_cast<int8_t>(e.exps[b] >> 8);
+            const float rb = reference - static_cast<float>(ev);
+            float w[8], sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = exp2_fast(fmaf(sc[b / 2][8 * (b % 2) + j], c[b], -rb));
+                sum += w[j];
+            }
+            l = fmaf(sum, power(-ev), l);
+            f16x8 wh, wl;
+            split_terms<TWO>(wh, wl, w);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const f16x8 x = *reinterpret_cast<const f16x8 *>(v + (2 * b * D + 32 * d) * 16);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, acc[d], 0, 0, 0);
+                if constexpr (TWO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, acc[d], 0, 0, 0);
+            }
+        }
+        if (__builtin_expect(any_nan, 0)) {
+            // Count the NaN values that each row sees with a product of ones (0x38 is 1.0 in e4m3); V's bytes are read again.
+#pragma unroll 1
+            for (int b = 0; b < 4; ++b) {
+                const int base = key0 + 16 * b + 8 * h;
+                const bool here = !((e.absent >> b) & 1u);
+                const uint32_t seen = here ? bit_range(low - base, high - base - 1) : 0u, held = here ? bit_range(0, t.vis.length - base - 1) : 0u;
+                f16x8 sees;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sees[j] = static_cast<_Float16>((seen >> j) & 1u ? 1.0f : 0.0f);
+                const int64_t vb = max(b == 0 ? e.places[0] : b == 1 ? e.places[1] : b == 2 ? e.places[2] : e.places[3], 0);
+                const uint8_t *const bytes = a.cache.values + vb * (kBlockTokens * D) + col * 16 + 8 * h;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const u32x2 y = *reinterpret_cast<const u32x2 *>(bytes + 32 * d * 16);
+                    const f32x16 hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen(nan_bytes(y[0] & byte_mask(held)) & 0x38383838u,
+                            nan_bytes(y[1] & byte_mask(held >> 4)) & 0x38383838u), sees, f32x16{}, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[d][j] = hits[j] > 0.0f ? NAN : acc[d][j];
+                    __builtin_amdgcn_sched_barrier(0); // one tile of counts at a time
+                }
+            }
+        }
+    };
+
+    Scales now{}, next{}, after{};
+    if (steps > 0) {
+        load(now, 0);
+        stage(0, now.absent);
+        if (steps > 1) load(next, 1);
+    }
+    __syncthreads();
+    for (int index = 0; index < steps; ++index) {
+        if (index + 1 < steps) stage(index + 1, next.absent);
+        if (index + 2 < steps) load(after, index + 2);
+        compute(index, now);
+        __syncthreads();
+        now = next;
+        next = after;
+    }
+
+    l = halves_sum(l);
+    m = halves_max(m);
+    if (!used) return;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int f = 32 * d + 8 * u + 4 * h;
+            const float o[4] = {acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
+            if (t.chunks <= 1) {
+                finish_row<T, VEC>(a, t.s.row0 + i, query_head, f, o, l, M, m, f == 0);
+            } else {
+                const Partial p = partial_of<D>(a, part, slot, r);
+                *reinterpret_cast<f32x4 *>(p.acc + f) = f32x4{o[0], o[1], o[2], o[3]};
+                if (f == 0) *reinterpret_cast<f32x4 *>(p.stats) = f32x4{M, l, m, 0.0f};
+            }
+        }
     }
 }
 
-template<int T, int D, int NQ, bool VEC>
+// Joins the chunks of a tile, in an order that their number fixes. D / 4 lanes hold a row's features; the other lanes of a wave,
+// and for many chunks the other waves of the workgroup, take chunks of their own with a running reference and are merged at the end.
+// WAVES: waves that share a row.
+template<int T, int D, bool VEC, int WAVES>
+__global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForwardArgs a, const ForwardPart part) {
+    constexpr int LANES = D / 4, SIDE = kWave / LANES; // chunks side by side in a wave
+    constexpr int ROWS = kWaves / WAVES;               // rows of a workgroup
+    __shared__ float merged[kWaves][4 * LANES + 4];
+    const int heads = a.cache.heads, group = a.query_heads / heads;
+    const uint32_t row_groups = part.rows / ROWS, pair = blockIdx.x / row_groups, unit = pair / heads;
+    const int head = static_cast<int>(pair - unit * heads);
+    const Tile t = tile_of(a, part, unit, group);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
+    const int first_row = static_cast<int>(blockIdx.x - pair * row_groups) * ROWS;
+    if (t.chunks <= 1 || first_row >= t.rows) return;
+    const int r = first_row + wave / WAVES, f = 4 * (lane % LANES);
+    float reference = -INFINITY, most = -INFINITY, sum = 0.0f, o[4] = {};
+    if (r < t.rows) {
+        const int64_t slot = static_cast<int64_t>(pair) * part.chunks;
+#pragma unroll 4
+        for (int c = (wave % WAVES) * SIDE + lane / LANES; c < t.chunks; c += WAVES * SIDE) {
+            const Partial p = partial_of<D>(a, part, slot + c, r);
+            const f32x4 s = *reinterpret_cast<const f32x4 *>(p.stats), x = *reinterpret_cast<const f32x4 *>(p.acc + f);
+            const float raised = fmaxf(reference, s[0]);
+            const float old = reference == raised ? 1.0f : exp2_fast(reference - raised), add = s[0] == raised ? 1.0f : exp2_fast(s[0] - raised);
+            reference = raised;
+            most = fmaxf(most, s[2]);
+            sum = fmaf(s[1], add, sum * old);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], add, o[j] * old);
+        }
+    }
+    auto merge = [&](const float other_reference, const float other_most, const float other_sum, const float (&x)[4]) __attribute__((always_inline)) {
+        const float raised = fmaxf(reference, other_reference);
+        const float old = reference == raised ? 1.0f : exp2_fast(reference - raised),
+                    add = other_reference == raised ? 1.0f : exp2_fast(other_reference - raised);
+        reference = raised;
+        most = fmaxf(most, other_most);
+        // The product of the earlier part and the later part in one order for both lanes: a sum of two is symmetric.
+        sum = sum * old + other_sum * add;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = o[j] * old + x[j] * add;
+    };
+#pragma unroll
+    for (int m = LANES; m < kWave; m <<= 1) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __shfl_xor(o[j], m);
+        merge(__shfl_xor(reference, m), __shfl_xor(most, m), __shfl_xor(sum, m), x);
+    }
+    if constexpr (WAVES > 1) {
+        if (lane < LANES) {
+            *reinterpret_cast<f32x4 *>(&merged[wave][f]) = f32x4{o[0], o[1], o[2], o[3]};
+            if (f == 0) *reinterpret_cast<f32x4 *>(&merged[wave][4 * LANES]) = f32x4{reference, most, sum, 0.0f};
+        }
+        __syncthreads();
+        if (wave % WAVES != 0) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) {
+            const f32x4 s = *reinterpret_cast<const f32x4 *>(&merged[wave + w][4 * LANES]);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&merged[wave + w][f]);
+            const float x[4] = {y[0], y[1], y[2], y[3]};
+            merge(s[0], s[1], s[2], x);
+        }
+    }
+    if (r >= t.rows || lane >= LANES) return;
+    const int flat = t.row0 + r, token = flat / group;
+    finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, o, sum, reference, most, f == 0);
+}
+
+template<int T, int D, bool VEC>
+void launch_join(const CacheForwardArgs &a, const ForwardPart &part, const uint32_t pairs, hipStream_t stream) {
+    // Many chunks: the waves of a workgroup share a row.
+    if (part.chunks > 8)
+        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, kWaves>), dim3(pairs * part.rows), dim3(kThreads), 0, stream, a, part);
+    else
+        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, 1>), dim3(pairs * (part.rows / kWaves)), dim3(kThreads), 0, stream, a, part);
+}
+
+template<int T, int D, bool VEC>
 void launch(const CacheForwardArgs &a, const ForwardPlan &plan, hipStream_t stream) {
-    const uint32_t pairs = static_cast<uint32_t>(plan.units) * a.cache.heads;
-    hipLaunchKernelGGL((cache_attention_kernel<T, D, NQ, VEC>), dim3(pairs * plan.chunks), dim3(kThreads), 0, stream, a, plan);
-    if (plan.chunks > 1) hipLaunchKernelGGL((cache_join_kernel<T, D, VEC>), dim3(pairs), dim3(kThreads), 0, stream, a, plan);
+    if (plan.large.units > 0) {
+        const uint32_t pairs = static_cast<uint32_t>(plan.large.units) * a.cache.heads;
+        hipLaunchKernelGGL((cache_attention_large_kernel<T, D, VEC>), dim3(pairs * plan.large.chunks), dim3(kThreads), 0, stream, a, plan.large);
+        if (plan.large.chunks > 1) launch_join<T, D, VEC>(a, plan.large, pairs, stream);
+    }
+    if (plan.small.units > 0) {
+        const uint32_t pairs = static_cast<uint32_t>(plan.small.units) * a.cache.heads;
+        if (plan.small.rows == 16)
+            hipLaunchKernelGGL((cache_attention_kernel<T, D, 1, VEC>), dim3(pairs * plan.small.chunks), dim3(kThreads), 0, stream, a, plan.small);
+        else
+            hipLaunchKernelGGL((cache_attention_kernel<T, D, 2, VEC>), dim3(pairs * plan.small.chunks), dim3(kThreads), 0, stream, a, plan.small);
+        if (plan.small.chunks > 1) launch_join<T, D, VEC>(a, plan.small, pairs, stream);
+    }
 }
 
 template<int T, int D>
 void dispatch(const CacheForwardArgs &a, const ForwardPlan &plan, const bool vec, hipStream_t stream) {
-    if (plan.rows == 16) {
-        if (vec) launch<T, D, 1, true>(a, plan, stream);
-        else launch<T, D, 1, false>(a, plan, stream);
-    } else {
-        if (vec) launch<T, D, 2, true>(a, plan, stream);
-        else launch<T, D, 2, false>(a, plan, stream);
-    }
+    if (vec) launch<T, D, true>(a, plan, stream);
+    else launch<T, D, false>(a, plan, stream);
 }
 
 template<int T>
@@ -490,8 +848,9 @@ void dispatch(const int width, const CacheForwardArgs &a, const ForwardPlan &pla
 } // namespace
 
 hipError_t launch_cache_forward(const int width, const CacheForwardArgs &a, const ForwardPlan &plan, hipStream_t stream) {
-    if (plan.units == 0) return hipSuccess;
-    if (static_cast<long long>(plan.units) * a.cache.heads * plan.chunks >= (1ll << 32) / kThreads) return hipErrorInvalidValue;
+    for (const ForwardPart *part : {&plan.small, &plan.large}) // threads of a launch, of the kernel and of the join
+        if (static_cast<long long>(part->units) * a.cache.heads * std::max(part->chunks, part->rows) >= (1ll << 32) / kThreads)
+            return hipErrorInvalidValue;
     const int unit = a.dtype == kFloat32 ? 4 : 8;
     auto fits = [&](const void *p, const rocmkernels_strides &s) {
         return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (s.head % unit) == 0 && (s.token % unit) == 0;

@@ -155,6 +155,17 @@ struct Sequence {
     uint32_t base;      // the first unit that belongs to it
 };
 
+__device__ __forceinline__ Sequence sequence_at(const SequenceView &s, const int b) {
+    Sequence r;
+    r.b = b;
+    r.row0 = clamped(s.starts[b], 0, s.tokens);
+    r.count = max(0, clamped(s.starts[b + 1], 0, s.tokens) - r.row0);
+    r.length = clamped(s.lengths[b], 0, kLengthLimit);
+    r.first = r.length - r.count;
+    r.base = 0;
+    return r;
+}
+
 // The sequence that unit `unit` belongs to (cache_plan.hpp). A sequence's first unit ascends with b, so each lane of the wave tests
 // one of 64 spaced sequences and a ballot gives the last whose base is not past the unit: one load per lane and round, two rounds
 // for up to 4096 sequences (a binary search has a dependent load for each bit).
@@ -171,12 +182,7 @@ __device__ __forceinline__ Sequence find_sequence(const SequenceView &s, const u
         low += hit * step;
         span = min(step, span - hit * step);
     }
-    Sequence r;
-    r.b = low;
-    r.row0 = clamped(s.starts[low], 0, s.tokens);
-    r.count = max(0, clamped(s.starts[low + 1], 0, s.tokens) - r.row0);
-    r.length = clamped(s.lengths[low], 0, kLengthLimit);
-    r.first = r.length - r.count;
+    Sequence r = sequence_at(s, low);
     r.base = unit_base(r.row0, low, mul, add, div);
     return r;
 }

@@ -48,34 +48,65 @@ inline long long page_units(const int tokens, const int batch, const int size) {
     return (tokens + static_cast<long long>(batch) * (2 * size - 2)) / size;
 }
 
-// Rows of a sequence are flattened to (row, query head of the group) and cut into tiles of `rows`; the keys a tile sees are cut into
-// chunks of `chunk_steps` steps, `chunks` at most.
+// One launch of the attention kernels. Rows of a sequence are flattened to (row, query head of the group) and cut into tiles of
+// `rows`; the keys a tile sees are cut into chunks of `chunk_steps` steps, `chunks` at most. A part takes the sequences that have
+// between `least` and `most` flattened rows; with `direct` every sequence has that many units, otherwise they are searched.
+struct ForwardPart {
+    int rows, units, direct, least, most, chunk_steps, chunks;
+    size_t workspace;   // bytes: one partial result for each chunk of each tile
+    size_t workspace_at; // where they start
+};
+
+// A call: tiles of few rows stream the keys for themselves (`small`), tiles of many rows share them (`large`).
 struct ForwardPlan {
-    int rows, units, chunk_steps, chunks;
+    ForwardPart small, large;
     size_t workspace;      // bytes this call needs
     size_t workspace_most; // and with any smaller window
 };
 
-inline ForwardPlan plan_cache_forward(const int width, const int dtype, const SequenceView &s, const int heads, const int query_heads,
-        const int max_keys, const int radius) {
-    (void)dtype;
-    ForwardPlan p;
+constexpr int kSmallRows = 32;  // sequences of up to this many flattened rows are small work where both kinds may be
+constexpr int kLargeTile = 128; // rows of a large tile
+
+inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, const int heads, const int query_heads, const int max_keys,
+        const int radius) {
     const int group = query_heads / heads;
     const long long flat = static_cast<long long>(s.tokens) * group;
-    p.rows = flat <= 16ll * s.batch ? 16 : 32;
-    p.units = static_cast<int>(row_units(flat, s.batch, p.rows));
-    // The keys that a tile may see: all, or its window.
-    long long span = max_keys;
-    if (radius >= 0) span = std::min(span, 2ll * radius + 1 + (p.rows + group - 1) / group + kStep);
-    const long long steps = (span + kStep - 1) / kStep;
-    const long long pairs = static_cast<long long>(p.units) * heads;
-    const long long wanted = (2048 + pairs - 1) / std::max(pairs, 1ll);
-    const long long chunks = std::min(wanted, std::max(1ll, steps / 8)); // grows with the keys and the window
-    p.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks);
-    p.chunks = static_cast<int>((steps + p.chunk_steps - 1) / p.chunk_steps);
-    const size_t chunk_bytes = static_cast<size_t>(pairs) * p.rows * (width + 4) * sizeof(float);
-    p.workspace = p.chunks > 1 ? chunk_bytes * p.chunks : 0;
-    p.workspace_most = chunks > 1 ? chunk_bytes * chunks : 0;
+    ForwardPlan p{};
+    size_t most = 0;
+    auto cut = [&](ForwardPart &part, const long long workgroups, const int least_steps) {
+        // The keys that a tile may see: all, or its window.
+        long long span = max_keys;
+        if (radius >= 0) span = std::min(span, 2ll * radius + 1 + (part.rows + group - 1) / group + kStep);
+        const long long steps = (span + kStep - 1) / kStep;
+        const long long pairs = static_cast<long long>(part.units) * heads;
+        const long long wanted = (workgroups + pairs - 1) / std::max(pairs, 1ll);
+        const long long chunks = std::min(wanted, std::max(1ll, steps / least_steps)); // grows with the keys and the window
+        part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks);
+        part.chunks = static_cast<int>((steps + part.chunk_steps - 1) / part.chunk_steps);
+        const size_t chunk_bytes = static_cast<size_t>(pairs) * part.rows * (width + 4) * sizeof(float);
+        part.workspace = part.chunks > 1 ? chunk_bytes * part.chunks : 0;
+        part.workspace_at = p.workspace;
+        p.workspace += part.workspace;
+        most += chunks > 1 ? chunk_bytes * chunks : 0;
+    };
+    // Batches whose sequences have a few rows on average are small work throughout, whatever a single sequence has.
+    const bool small_only = flat <= 16ll * s.batch || flat <= kSmallRows;
+    if (!small_only) {
+        p.large.rows = kLargeTile;
+        p.large.units = static_cast<int>(row_units(flat, s.batch, kLargeTile));
+        p.large.least = s.batch > 1 ? kSmallRows + 1 : 1;
+        p.large.most = 0x7fffffff;
+        cut(p.large, 512, 8);
+    }
+    if (small_only || s.batch > 1) {
+        p.small.rows = small_only && flat <= 16ll * s.batch ? 16 : 32;
+        p.small.direct = small_only ? 0 : 1; // one tile holds all rows of a small sequence
+        p.small.units = small_only ? static_cast<int>(row_units(flat, s.batch, p.small.rows)) : s.batch;
+        p.small.least = 1;
+        p.small.most = small_only ? 0x7fffffff : kSmallRows;
+        cut(p.small, 2048, 8);
+    }
+    p.workspace_most = most;
     return p;
 }
 

@@ -70,13 +70,30 @@ int main() {
             if (starts[b + 1] > starts[b]) check(search(starts, batch, tokens, starts[b + 1] - 1, 1, 0, 1) == b, "search for a token");
         // Plans.
         const rk::SequenceView s{nullptr, nullptr, nullptr, batch, tokens, 1, 1};
-        const int heads = pick(1, 12), keys = pick(0, 2) ? pick(1, 5000) : pick(1, 200000), width = 32 << pick(0, 2), dtype = pick(0, 2);
-        const size_t whole = rk::plan_cache_forward(width, dtype, s, heads, heads * group, keys, -1).workspace_most;
+        const int heads = pick(1, 12), keys = pick(0, 2) ? pick(1, 5000) : pick(1, 200000), width = 32 << pick(0, 2);
+        const size_t whole = rk::plan_cache_forward(width, s, heads, heads * group, keys, -1).workspace_most;
         for (const int radius : {-1, 0, 1, 100, 777, 5000, 100000}) {
-            const rk::ForwardPlan p = rk::plan_cache_forward(width, dtype, s, heads, heads * group, keys, radius);
-            check(p.rows <= rk::kMaxRows && p.chunks >= 1 && p.chunk_steps >= 1, "plan");
+            const rk::ForwardPlan p = rk::plan_cache_forward(width, s, heads, heads * group, keys, radius);
             check(p.workspace <= whole, "a window needs more workspace than the whole");
-            if (radius < 0) check(static_cast<long long>(p.chunks) * p.chunk_steps * 64 >= keys, "chunks do not cover the keys");
+            check(p.small.workspace + p.large.workspace == p.workspace, "parts of the workspace");
+            for (const rk::ForwardPart *part : {&p.small, &p.large}) {
+                if (part->units == 0) continue;
+                check(part->rows > 0 && part->rows <= rk::kMaxRows && part->chunks >= 1 && part->chunk_steps >= 1, "part");
+                check(part->workspace_at + part->workspace <= p.workspace, "a part lies behind the workspace");
+                if (radius < 0) check(static_cast<long long>(part->chunks) * part->chunk_steps * rk::kStep >= keys, "chunks do not cover the keys");
+            }
+            // Every number of rows belongs to exactly one part, and a part with one unit a sequence holds all its rows.
+            for (int b = 0; b < batch; b += 1 + batch / 20) {
+                const int rows = (starts[b + 1] - starts[b]) * group;
+                if (rows == 0) continue;
+                int parts = 0;
+                for (const rk::ForwardPart *part : {&p.small, &p.large}) {
+                    const bool takes = part->units > 0 && rows >= part->least && rows <= part->most;
+                    parts += takes;
+                    if (takes && part->direct) check(rows <= part->direct * part->rows, "a direct part leaves rows out");
+                }
+                check(parts == 1, "rows of no part or of two");
+            }
         }
     }
     std::printf("%d failure(s)\n", failures);
