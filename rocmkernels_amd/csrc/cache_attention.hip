@@ -612,11 +612,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         const uint8_t *const k = staged[index & 1] + token_of_row * 16 + h * K_CHUNK;
         const uint8_t *const v = staged[index & 1] + K_BYTES + (h * D + col) * 16;
         f32x16 sc[2];
+        sc[0] = sc[1] = f32x16{};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            sc[n] = f32x16{};
+        for (int c = 0; c < KC; ++c) { // two independent chains
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
+            for (int n = 0; n < 2; ++n) {
                 const f16x8 w = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK) + n * 512);
                 sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[c], sc[n], 0, 0, 0);
                 if constexpr (TWO) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[c], sc[n], 0, 0, 0);
@@ -700,6 +700,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         }
     };
 
+    // The rows of q are here before the first step is asked for: a wait for them inside the loop would be one for the newest loads.
+    __builtin_amdgcn_s_waitcnt(0x0f70); // vmcnt 0
     Scales now{}, next{}, after{};
     if (steps > 0) {
         load(now, 0);
@@ -738,72 +740,71 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 
 // Joins the chunks of a tile, in an order that their number fixes. D / 4 lanes hold a row's features; the other lanes of a wave,
 // and for many chunks the other waves of the workgroup, take chunks of their own with a running reference and are merged at the end.
-// WAVES: waves that share a row.
+// WAVES: waves that share a row; with one, a wave joins kJoinRows / 4 rows in turn.
+constexpr int kJoinRows = 16;
+
+struct Joined {
+    float reference = -INFINITY, most = -INFINITY, sum = 0.0f, o[4] = {};
+    __device__ __forceinline__ void add(const float other_reference, const float other_most, const float other_sum, const float (&x)[4]) {
+        const float raised = fmaxf(reference, other_reference);
+        const float mine = reference == raised ? 1.0f : exp2_fast(reference - raised),
+                    theirs = other_reference == raised ? 1.0f : exp2_fast(other_reference - raised);
+        reference = raised;
+        most = fmaxf(most, other_most);
+        sum = sum * mine + other_sum * theirs; // a sum of two products: the same for both lanes of an exchange
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = o[j] * mine + x[j] * theirs;
+    }
+};
+
 template<int T, int D, bool VEC, int WAVES>
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForwardArgs a, const ForwardPart part) {
     constexpr int LANES = D / 4, SIDE = kWave / LANES; // chunks side by side in a wave
-    constexpr int ROWS = kWaves / WAVES;               // rows of a workgroup
+    constexpr int ROWS = WAVES == 1 ? kJoinRows : 1;   // rows of a workgroup
     __shared__ float merged[kWaves][4 * LANES + 4];
     const int heads = a.cache.heads, group = a.query_heads / heads;
     const uint32_t row_groups = part.rows / ROWS, pair = blockIdx.x / row_groups, unit = pair / heads;
     const int head = static_cast<int>(pair - unit * heads);
     const Tile t = tile_of(a, part, unit, group);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
-    const int first_row = static_cast<int>(blockIdx.x - pair * row_groups) * ROWS;
+    const int first_row = static_cast<int>(blockIdx.x - pair * row_groups) * ROWS, f = 4 * (lane % LANES);
+    const int64_t slot = static_cast<int64_t>(pair) * part.chunks;
     if (t.chunks <= 1 || first_row >= t.rows) return;
-    const int r = first_row + wave / WAVES, f = 4 * (lane % LANES);
-    float reference = -INFINITY, most = -INFINITY, sum = 0.0f, o[4] = {};
-    if (r < t.rows) {
-        const int64_t slot = static_cast<int64_t>(pair) * part.chunks;
+    for (int r = first_row + (WAVES == 1 ? wave : 0); r < min(first_row + ROWS, t.rows); r += kWaves) {
+        Joined row;
 #pragma unroll 4
-        for (int c = (wave % WAVES) * SIDE + lane / LANES; c < t.chunks; c += WAVES * SIDE) {
+        for (int c = (WAVES == 1 ? 0 : wave * SIDE) + lane / LANES; c < t.chunks; c += WAVES * SIDE) {
             const Partial p = partial_of<D>(a, part, slot + c, r);
-            const f32x4 s = *reinterpret_cast<const f32x4 *>(p.stats), x = *reinterpret_cast<const f32x4 *>(p.acc + f);
-            const float raised = fmaxf(reference, s[0]);
-            const float old = reference == raised ? 1.0f : exp2_fast(reference - raised), add = s[0] == raised ? 1.0f : exp2_fast(s[0] - raised);
-            reference = raised;
-            most = fmaxf(most, s[2]);
-            sum = fmaf(s[1], add, sum * old);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], add, o[j] * old);
-        }
-    }
-    auto merge = [&](const float other_reference, const float other_most, const float other_sum, const float (&x)[4]) __attribute__((always_inline)) {
-        const float raised = fmaxf(reference, other_reference);
-        const float old = reference == raised ? 1.0f : exp2_fast(reference - raised),
-                    add = other_reference == raised ? 1.0f : exp2_fast(other_reference - raised);
-        reference = raised;
-        most = fmaxf(most, other_most);
-        // The product of the earlier part and the later part in one order for both lanes: a sum of two is symmetric.
-        sum = sum * old + other_sum * add;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = o[j] * old + x[j] * add;
-    };
-#pragma unroll
-    for (int m = LANES; m < kWave; m <<= 1) {
-        float x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __shfl_xor(o[j], m);
-        merge(__shfl_xor(reference, m), __shfl_xor(most, m), __shfl_xor(sum, m), x);
-    }
-    if constexpr (WAVES > 1) {
-        if (lane < LANES) {
-            *reinterpret_cast<f32x4 *>(&merged[wave][f]) = f32x4{o[0], o[1], o[2], o[3]};
-            if (f == 0) *reinterpret_cast<f32x4 *>(&merged[wave][4 * LANES]) = f32x4{reference, most, sum, 0.0f};
-        }
-        __syncthreads();
-        if (wave % WAVES != 0) return;
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) {
-            const f32x4 s = *reinterpret_cast<const f32x4 *>(&merged[wave + w][4 * LANES]);
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(&merged[wave + w][f]);
+            const f32x4 s = *reinterpret_cast<const f32x4 *>(p.stats), y = *reinterpret_cast<const f32x4 *>(p.acc + f);
             const float x[4] = {y[0], y[1], y[2], y[3]};
-            merge(s[0], s[1], s[2], x);
+            row.add(s[0], s[2], s[1], x);
+        }
+#pragma unroll
+        for (int m = LANES; m < kWave; m <<= 1) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = __shfl_xor(row.o[j], m);
+            row.add(__shfl_xor(row.reference, m), __shfl_xor(row.most, m), __shfl_xor(row.sum, m), x);
+        }
+        if constexpr (WAVES > 1) {
+            if (lane < LANES) {
+                *reinterpret_cast<f32x4 *>(&merged[wave][f]) = f32x4{row.o[0], row.o[1], row.o[2], row.o[3]};
+                if (f == 0) *reinterpret_cast<f32x4 *>(&merged[wave][4 * LANES]) = f32x4{row.reference, row.most, row.sum, 0.0f};
+            }
+            __syncthreads();
+            if (wave != 0) return;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) {
+                const f32x4 s = *reinterpret_cast<const f32x4 *>(&merged[w][4 * LANES]), y = *reinterpret_cast<const f32x4 *>(&merged[w][f]);
+                const float x[4] = {y[0], y[1], y[2], y[3]};
+                row.add(s[0], s[1], s[2], x);
+            }
+        }
+        if (lane < LANES) {
+            const int flat = t.row0 + r, token = flat / group;
+            finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, row.o, row.sum, row.reference, row.most, f == 0);
         }
     }
-    if (r >= t.rows || lane >= LANES) return;
-    const int flat = t.row0 + r, token = flat / group;
-    finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, o, sum, reference, most, f == 0);
 }
 
 template<int T, int D, bool VEC>
@@ -812,7 +813,7 @@ void launch_join(const CacheForwardArgs &a, const ForwardPart &part, const uint3
     if (part.chunks > 8)
         hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, kWaves>), dim3(pairs * part.rows), dim3(kThreads), 0, stream, a, part);
     else
-        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, 1>), dim3(pairs * (part.rows / kWaves)), dim3(kThreads), 0, stream, a, part);
+        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, 1>), dim3(pairs * (part.rows / kJoinRows)), dim3(kThreads), 0, stream, a, part);
 }
 
 template<int T, int D, bool VEC>

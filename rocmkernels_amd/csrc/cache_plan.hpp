@@ -99,9 +99,9 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         cut(p.large, 512, 8);
     }
     if (small_only || s.batch > 1) {
-        p.small.rows = small_only && flat <= 16ll * s.batch ? 16 : 32;
-        p.small.direct = small_only ? 0 : 1; // one tile holds all rows of a small sequence
-        p.small.units = small_only ? static_cast<int>(row_units(flat, s.batch, p.small.rows)) : s.batch;
+        p.small.rows = 16;
+        p.small.direct = small_only ? 0 : kSmallRows / 16;
+        p.small.units = small_only ? static_cast<int>(row_units(flat, s.batch, 16)) : s.batch * p.small.direct;
         p.small.least = 1;
         p.small.most = small_only ? 0x7fffffff : kSmallRows;
         cut(p.small, 2048, 8);
