@@ -5,10 +5,10 @@
 // costs e4m3 nothing, as a float's relative step does not depend on the scale, and makes every step exact but the one rounding: x * 2^-e
 // is exact, and earlier rows keep their values when the scale grows (but for subnormals).
 //
-// One job per (page, head, K or V), because the scale needs all the new rows of the page before the first byte is written: a
-// workgroup of four waves where sequences bring many rows, one wave (four jobs to a workgroup) where they bring a few. A job
+// One job per (page, head, K or V), because the scale needs all the new rows of the page before the first byte is written: a wave
+// (four jobs to a workgroup) where sequences bring a few rows or the page fits a wave's registers, four waves otherwise. A job
 // holds its rotated values in registers between the two passes (rows beyond what fits are read again, from L2). Query rows are
-// rotated by further workgroups of the same launch, a wave per token, so that all reads of a call are in flight together.
+// rotated by further workgroups of the same launch, so that all reads of a call are in flight together.
 #include "cache_device.hpp"
 #include "cache_launch.hpp"
 
@@ -16,38 +16,33 @@ namespace rk {
 
 namespace {
 
-// Sixteen values of a row: columns c .. c + 7 and their partners c + D / 2 .. c + D / 2 + 7, rotated if there are tables.
-// Each product is rounded before the sum, as rotary.hip does (the library is built with -ffp-contract=off).
-template<int T, int D, bool VEC>
-__device__ __forceinline__ void load_turned(float (&y)[16], const void *x, const int64_t row, const int c, const float *cos,
-        const float *sin, const int64_t cos_row, const int64_t sin_row) {
+// Sixteen values of a row: columns c .. c + 7 and their partners c + D / 2 .. c + D / 2 + 7.
+struct Pairs {
     float lo[8], hi[8];
-    load8<T, VEC>(lo, x, row + c);
-    load8<T, VEC>(hi, x, row + c + D / 2);
-    if (cos) {
-        float cl[8], ch[8], sl[8], sh[8];
-        load8<kFloat32, VEC>(cl, cos, cos_row + c);
-        load8<kFloat32, VEC>(ch, cos, cos_row + c + D / 2);
-        load8<kFloat32, VEC>(sl, sin, sin_row + c);
-        load8<kFloat32, VEC>(sh, sin, sin_row + c + D / 2);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            y[i] = lo[i] * cl[i] - hi[i] * sl[i];
-            y[8 + i] = hi[i] * ch[i] + lo[i] * sh[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            y[i] = lo[i];
-            y[8 + i] = hi[i];
-        }
-    }
+};
+template<int T, int D, bool VEC>
+__device__ __forceinline__ Pairs load_pairs(const void *x, const int64_t element) {
+    Pairs p;
+    load8<T, VEC>(p.lo, x, element);
+    load8<T, VEC>(p.hi, x, element + D / 2);
+    return p;
 }
 
-template<int N>
-__device__ __forceinline__ float largest(float most, const float (&x)[N]) {
+// Rotated by a row of the tables. Each product is rounded before the sum, as rotary.hip does (the library is built with
+// -ffp-contract=off).
+__device__ __forceinline__ Pairs turned(const Pairs &x, const Pairs &cos, const Pairs &sin) {
+    Pairs y;
 #pragma unroll
-    for (int i = 0; i < N; ++i) most = fmaxf(most, isfinite(x[i]) ? fabsf(x[i]) : 0.0f);
+    for (int i = 0; i < 8; ++i) {
+        y.lo[i] = x.lo[i] * cos.lo[i] - x.hi[i] * sin.lo[i];
+        y.hi[i] = x.hi[i] * cos.hi[i] + x.lo[i] * sin.hi[i];
+    }
+    return y;
+}
+
+__device__ __forceinline__ float largest(float most, const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, isfinite(x[i]) ? fabsf(x[i]) : 0.0f);
     return most;
 }
 
@@ -72,16 +67,16 @@ __device__ __forceinline__ void job_sync() {
     else wave_lds_sync();
 }
 
-// The rows of one sequence that land on one page.
+// The rows of one sequence that land on one page. Nothing of it depends on the page's number, so the rows are on their way before the
+// table has answered.
 struct PageRows {
     int slot0, count;  // new rows take slots slot0 .. slot0 + count - 1
     int64_t row;       // packed row of slot 0 (counted back from the first new row)
     int64_t position;  // position of slot 0
-    int64_t cell;      // page * heads + head
+    int64_t cell;      // page * heads + head; negative: no page
 };
 
 // New scale exponent of the page for one of its halves; writes it.
-template<int W>
 __device__ __forceinline__ int settle_scale(const AppendArgs &a, const PageRows &p, const int which, const float most, const int before,
         const int thread) {
     int e = exponent_for(most);
@@ -94,31 +89,32 @@ template<int T, int D, bool VEC, int W>
 __device__ __forceinline__ void append_keys(const AppendArgs &a, const PageRows &p, const int head, const int thread, float *shared) {
     constexpr int CG = D / 16;          // threads of a row
     constexpr int THREADS = W * kWave;
-    constexpr int KEPT = 4;             // a full page of 128 tokens at D = 128 with four waves; 32 tokens with one
-    const int before = scale_exponent(a.cache.scales[2 * p.cell]);
+    constexpr int KEPT = 4;             // a page of 128 tokens at D = 128 with four waves, 4096 values with one
     const int items = p.count * CG;
-    auto load = [&](float (&y)[16], const int item) __attribute__((always_inline)) {
-        const int slot = p.slot0 + item / CG;
+    auto load = [&](const int item) __attribute__((always_inline)) {
+        const int slot = p.slot0 + item / CG, c = 8 * (item % CG);
         const int64_t at = p.position + slot;
-        load_turned<T, D, VEC>(y, a.k, (p.row + slot) * a.ks.token + static_cast<int64_t>(head) * a.ks.head, 8 * (item % CG), a.cos, a.sin,
-                at * a.cs.token, at * a.ss.token);
+        const Pairs x = load_pairs<T, D, VEC>(a.k, (p.row + slot) * a.ks.token + static_cast<int64_t>(head) * a.ks.head + c);
+        if (!a.cos) return x;
+        return turned(x, load_pairs<kFloat32, D, VEC>(a.cos, at * a.cs.token + c), load_pairs<kFloat32, D, VEC>(a.sin, at * a.ss.token + c));
     };
-    float kept[KEPT][16];
+    Pairs kept[KEPT];
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) {
         const int item = thread + i * THREADS;
         if (item < items) {
-            load(kept[i], item);
-            most = largest(most, kept[i]);
+            kept[i] = load(item);
+            most = largest(largest(most, kept[i].lo), kept[i].hi);
         }
     }
     for (int item = thread + KEPT * THREADS; item < items; item += THREADS) {
-        float y[16];
-        load(y, item);
-        most = largest(most, y);
+        const Pairs y = load(item);
+        most = largest(largest(most, y.lo), y.hi);
     }
-    const int e = settle_scale<W>(a, p, 0, job_max<W>(most, shared), before, thread);
+    if (p.cell < 0) return;
+    const int before = scale_exponent(a.cache.scales[2 * p.cell]);
+    const int e = settle_scale(a, p, 0, job_max<W>(most, shared), before, thread);
     uint8_t *const page = a.cache.keys + p.cell * a.cache.page_size * D;
     if (p.slot0 > 0 && e > before) { // rows in front of the new ones: whole rows, so none shares a byte with them
         const float factor = power(max(before - e, -126));
@@ -129,25 +125,21 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, const PageRows 
         }
     }
     const float factor = power(-e);
-    auto store = [&](const float (&y)[16], const int item) __attribute__((always_inline)) {
+    auto store = [&](const Pairs &y, const int item) __attribute__((always_inline)) {
         uint8_t *const row = page + (p.slot0 + item / CG) * D + 8 * (item % CG);
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = to_e4m3(y[4 * i] * factor, y[4 * i + 1] * factor, y[4 * i + 2] * factor, y[4 * i + 3] * factor);
-        *reinterpret_cast<u32x2 *>(row) = u32x2{w[0], w[1]};
-        *reinterpret_cast<u32x2 *>(row + D / 2) = u32x2{w[2], w[3]};
+        auto bytes = [&](const float (&x)[8]) __attribute__((always_inline)) {
+            return u32x2{to_e4m3(x[0] * factor, x[1] * factor, x[2] * factor, x[3] * factor),
+                    to_e4m3(x[4] * factor, x[5] * factor, x[6] * factor, x[7] * factor)};
+        };
+        *reinterpret_cast<u32x2 *>(row) = bytes(y.lo);
+        *reinterpret_cast<u32x2 *>(row + D / 2) = bytes(y.hi);
     };
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) {
         const int item = thread + i * THREADS;
         if (item < items) store(kept[i], item);
     }
-    for (int item = thread + KEPT * THREADS; item < items; item += THREADS) {
-        float y[16];
-        load(y, item);
-        store(y, item);
-    }
+    for (int item = thread + KEPT * THREADS; item < items; item += THREADS) store(load(item), item);
 }
 
 // V is stored with the 16 tokens of a block side by side for each feature, so a thread takes 4 tokens (slots 4q .. 4q + 3) by 8
@@ -155,6 +147,8 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, const PageRows 
 // the quads of a block that is not all new are stored from registers, byte by byte where a quad is not all new either.
 template<int D>
 constexpr int kBlockStride = D * 16 + D / 8 * 16; // LDS bytes of a block: 16 bytes of padding per 8 features keep the writes on distinct banks
+constexpr int kWavePage = 4096;                   // values of a page that one wave holds in registers, and stages
+constexpr int kStaged = kWaves * (kWavePage + kWavePage / 8); // four waves' pages, or one workgroup's of 128 tokens at D = 128
 
 template<int T, int D, bool VEC, int W>
 __device__ __forceinline__ void append_values(const AppendArgs &a, const PageRows &p, const int head, const int thread, float *shared,
@@ -162,7 +156,6 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, const PageRow
     constexpr int CG = D / 8;
     constexpr int THREADS = W * kWave;
     constexpr int KEPT = 2;
-    const int before = scale_exponent(a.cache.scales[2 * p.cell + 1]);
     const int end = p.slot0 + p.count;
     const int quad0 = p.slot0 / 4;
     const int items = ((end + 3) / 4 - quad0) * CG;
@@ -195,7 +188,9 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, const PageRow
 #pragma unroll
         for (int t = 0; t < 4; ++t) most = largest(most, y[t]);
     }
-    const int e = settle_scale<W>(a, p, 1, job_max<W>(most, shared), before, thread);
+    if (p.cell < 0) return;
+    const int before = scale_exponent(a.cache.scales[2 * p.cell + 1]);
+    const int e = settle_scale(a, p, 1, job_max<W>(most, shared), before, thread);
     uint8_t *const page = a.cache.values + p.cell * a.cache.page_size * D;
     if (p.slot0 > 0 && e > before) {
         // Dwords of 4 tokens; the last one may hold new slots too, whose bytes pass through and are written below.
@@ -209,9 +204,10 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, const PageRow
         job_sync<W>();
     }
     const float factor = power(-e);
+    const bool staging = W > 1 || a.cache.page_size * D <= kWavePage;
     auto store = [&](const float (&y)[4][8], const int item) __attribute__((always_inline)) {
         const int quad = quad0 + item / CG, block = quad / 4, d0 = 8 * (item % CG);
-        const bool whole = W > 1 && 16 * block >= p.slot0 && 16 * block + 16 <= end;
+        const bool whole = staging && 16 * block >= p.slot0 && 16 * block + 16 <= end;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t w = to_e4m3(y[0][i] * factor, y[1][i] * factor, y[2][i] * factor, y[3][i] * factor);
@@ -239,47 +235,58 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, const PageRow
         load(y, item);
         store(y, item);
     }
-    if constexpr (W > 1) {
-        __syncthreads();
-        const int block0 = (p.slot0 + 15) / 16, blocks = end / 16 - block0;
-        for (int i = thread; i < blocks * D; i += THREADS) {
-            const int block = block0 + i / D, d = i % D;
-            *reinterpret_cast<u32x4 *>(page + block * (16 * D) + d * 16) =
-                    *reinterpret_cast<const u32x4 *>(staged + block * kBlockStride<D> + d * 16 + (d / 8) * 16);
-        }
+    if (!staging) return;
+    job_sync<W>();
+    const int block0 = (p.slot0 + 15) / 16, blocks = end / 16 - block0;
+    for (int i = thread; i < blocks * D; i += THREADS) {
+        const int block = block0 + i / D, d = i % D;
+        *reinterpret_cast<u32x4 *>(page + block * (16 * D) + d * 16) =
+                *reinterpret_cast<const u32x4 *>(staged + block * kBlockStride<D> + d * 16 + (d / 8) * 16);
     }
 }
 
+// Tokens token .. token + count - 1, a wave. Neighbours mostly belong to one sequence, so it is searched once and then followed.
 template<int T, int D, bool VEC>
-__device__ __forceinline__ void rotate_queries(const AppendArgs &a, const int token) {
+__device__ __forceinline__ void rotate_queries(const AppendArgs &a, int token, const int count) {
     constexpr int CG = D / 16;
     if (token >= a.seqs.tokens) return;
-    const Sequence s = find_sequence(a.seqs, static_cast<uint32_t>(token), 1, 0, 1);
-    const int i = token - s.row0, position = s.first + i;
-    if (i < 0 || i >= s.count || position < 0 || position >= a.positions) return;
-    const int lane = threadIdx.x & (kWave - 1), c = 8 * (lane % CG);
-    for (int head = lane / CG; head < a.query_heads; head += kWave / CG) {
-        float y[16], lo[8], hi[8];
-        load_turned<T, D, VEC>(y, a.q, static_cast<int64_t>(token) * a.qs.token + static_cast<int64_t>(head) * a.qs.head, c, a.cos, a.sin,
-                static_cast<int64_t>(position) * a.cs.token, static_cast<int64_t>(position) * a.ss.token);
+    const int end = min(token + count, a.seqs.tokens), lane = threadIdx.x & (kWave - 1), c = 8 * (lane % CG);
+    Sequence s = find_sequence(a.seqs, static_cast<uint32_t>(token), 1, 0, 1);
+    for (; token < end; ++token) {
+        while (token >= s.row0 + s.count && s.b + 1 < a.seqs.batch) s = sequence_at(a.seqs, s.b + 1);
+        const int i = token - s.row0, position = s.first + i;
+        if (i < 0 || i >= s.count || position < 0 || position >= a.positions) continue;
+        const Pairs cos = load_pairs<kFloat32, D, VEC>(a.cos, static_cast<int64_t>(position) * a.cs.token + c);
+        const Pairs sin = load_pairs<kFloat32, D, VEC>(a.sin, static_cast<int64_t>(position) * a.ss.token + c);
+        constexpr int TOGETHER = T == kFloat32 ? 2 : 4, SIDE = kWave / CG; // heads a lane has under way, heads side by side
+        for (int head0 = lane / CG; head0 < a.query_heads; head0 += TOGETHER * SIDE) {
+            Pairs x[TOGETHER];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            lo[j] = y[j];
-            hi[j] = y[8 + j];
+            for (int j = 0; j < TOGETHER; ++j) {
+                const int head = min(head0 + j * SIDE, a.query_heads - 1);
+                x[j] = load_pairs<T, D, VEC>(a.q, static_cast<int64_t>(token) * a.qs.token + static_cast<int64_t>(head) * a.qs.head + c);
+            }
+#pragma unroll
+            for (int j = 0; j < TOGETHER; ++j) {
+                const int head = head0 + j * SIDE;
+                if (head >= a.query_heads) break;
+                const Pairs y = turned(x[j], cos, sin);
+                const int64_t to = static_cast<int64_t>(token) * a.os.token + static_cast<int64_t>(head) * a.os.head + c;
+                store_row<T, VEC>(a.oq, to, y.lo);
+                store_row<T, VEC>(a.oq, to + D / 2, y.hi);
+            }
         }
-        const int64_t to = static_cast<int64_t>(token) * a.os.token + static_cast<int64_t>(head) * a.os.head + c;
-        store_row<T, VEC>(a.oq, to, lo);
-        store_row<T, VEC>(a.oq, to + D / 2, hi);
     }
 }
 
 template<int T, int D, bool VEC, int W>
-__global__ __launch_bounds__(kThreads) void cache_append_kernel(const AppendArgs a, const uint32_t jobs, const uint32_t job_groups) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void cache_append_kernel(const AppendArgs a, const uint32_t jobs, const uint32_t job_groups,
+        const int tokens_a_wave) {
     __shared__ float shared[kWaves];
-    __shared__ __align__(16) uint8_t staged[W > 1 ? kMaxPage / 16 * kBlockStride<D> : 16];
+    __shared__ __align__(16) uint8_t staged[kStaged];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (blockIdx.x >= job_groups) {
-        rotate_queries<T, D, VEC>(a, static_cast<int>(blockIdx.x - job_groups) * kWaves + wave);
+        rotate_queries<T, D, VEC>(a, (static_cast<int>(blockIdx.x - job_groups) * kWaves + wave) * tokens_a_wave, tokens_a_wave);
         return;
     }
     const uint32_t job = W > 1 ? blockIdx.x : blockIdx.x * kWaves + wave;
@@ -293,14 +300,14 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(const AppendArgs
     const int low = max(max(s.first, 0), page_index * size), high = min(min(s.length, (page_index + 1) * size), a.positions);
     if (low >= high) return;
     const int page = a.seqs.table[static_cast<int64_t>(s.b) * a.seqs.table_stride + page_index];
-    if (page < 0 || page >= a.cache.pages) return;
     PageRows p;
     p.slot0 = low - page_index * size;
     p.count = high - low;
     p.position = static_cast<int64_t>(page_index) * size;
     p.row = s.row0 + (p.position - s.first);
-    p.cell = static_cast<int64_t>(page) * a.cache.heads + head;
-    if (rest & 1) append_values<T, D, VEC, W>(a, p, head, thread, shared, staged);
+    p.cell = page < 0 || page >= a.cache.pages ? -1 : static_cast<int64_t>(page) * a.cache.heads + head;
+    uint8_t *const own = staged + (W > 1 ? 0 : wave * (kStaged / kWaves));
+    if (rest & 1) append_values<T, D, VEC, W>(a, p, head, thread, shared, own);
     else append_keys<T, D, VEC, W>(a, p, head, thread, shared);
 }
 
@@ -309,14 +316,17 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 template<int T, int D, bool VEC, int W>
 void launch(const AppendArgs &a, const uint32_t jobs, hipStream_t stream) {
     const uint32_t job_groups = W > 1 ? jobs : (jobs + kWaves - 1) / kWaves;
-    const uint32_t query_groups = a.q ? static_cast<uint32_t>((static_cast<int64_t>(a.seqs.tokens) + kWaves - 1) / kWaves) : 0;
-    hipLaunchKernelGGL((cache_append_kernel<T, D, VEC, W>), dim3(job_groups + query_groups), dim3(kThreads), 0, stream, a, jobs, job_groups);
+    // A wave takes one token while tokens are few, more once every SIMD has several waves of them.
+    const int tokens_a_wave = a.seqs.tokens >= 8192 ? 4 : a.seqs.tokens >= 4096 ? 2 : 1, tokens = kWaves * tokens_a_wave;
+    const uint32_t query_groups = a.q ? static_cast<uint32_t>((static_cast<int64_t>(a.seqs.tokens) + tokens - 1) / tokens) : 0;
+    hipLaunchKernelGGL((cache_append_kernel<T, D, VEC, W>), dim3(job_groups + query_groups), dim3(kThreads), 0, stream, a, jobs, job_groups,
+            tokens_a_wave);
 }
 
 template<int T, int D>
 void dispatch(const AppendArgs &a, const bool vec, const uint32_t jobs, hipStream_t stream) {
-    // Few rows a sequence: a wave for each job.
-    if (a.seqs.tokens <= 8ll * a.seqs.batch) {
+    // Few rows a sequence, or a page that a wave holds in registers: a wave for each job.
+    if (a.seqs.tokens <= 8ll * a.seqs.batch || a.cache.page_size * D <= kWavePage) {
         if (vec) launch<T, D, true, 1>(a, jobs, stream);
         else launch<T, D, false, 1>(a, jobs, stream);
     } else {

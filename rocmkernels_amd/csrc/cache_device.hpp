@@ -155,25 +155,30 @@ struct Sequence {
     uint32_t base;      // the first unit that belongs to it
 };
 
-__device__ __forceinline__ Sequence sequence_at(const SequenceView &s, const int b) {
+__device__ __forceinline__ Sequence make_sequence(const int b, const int row0, const int end, const int length) {
     Sequence r;
     r.b = b;
-    r.row0 = clamped(s.starts[b], 0, s.tokens);
-    r.count = max(0, clamped(s.starts[b + 1], 0, s.tokens) - r.row0);
-    r.length = clamped(s.lengths[b], 0, kLengthLimit);
+    r.row0 = row0;
+    r.count = max(0, end - row0);
+    r.length = clamped(length, 0, kLengthLimit);
     r.first = r.length - r.count;
     r.base = 0;
     return r;
 }
 
+__device__ __forceinline__ Sequence sequence_at(const SequenceView &s, const int b) {
+    return make_sequence(b, clamped(s.starts[b], 0, s.tokens), clamped(s.starts[b + 1], 0, s.tokens), s.lengths[b]);
+}
+
 // The sequence that unit `unit` belongs to (cache_plan.hpp). A sequence's first unit ascends with b, so each lane of the wave tests
 // one of 64 spaced sequences and a ballot gives the last whose base is not past the unit: one load per lane and round, two rounds
-// for up to 4096 sequences (a binary search has a dependent load for each bit).
+// for up to 4096 sequences (a binary search has a dependent load for each bit). The last round's lanes hold neighbouring sequences,
+// with all that is known of them, so what it finds needs no further load.
 __device__ __forceinline__ Sequence find_sequence(const SequenceView &s, const uint32_t unit, const uint32_t mul, const uint32_t add,
         const uint32_t div) {
     const int lane = threadIdx.x & (kWave - 1);
     int low = 0, span = s.batch;
-    while (span > 1) {
+    while (span > kWave) {
         const int step = search_step(span);
         const int b = low + lane * step;
         const bool in = lane * step < span;
@@ -182,8 +187,14 @@ __device__ __forceinline__ Sequence find_sequence(const SequenceView &s, const u
         low += hit * step;
         span = min(step, span - hit * step);
     }
-    Sequence r = sequence_at(s, low);
-    r.base = unit_base(r.row0, low, mul, add, div);
+    const bool in = lane < span;
+    const int b = in ? low + lane : low;
+    const int start = clamped(s.starts[b], 0, s.tokens), end = clamped(s.starts[b + 1], 0, s.tokens), length = s.lengths[b];
+    const uint64_t reached = __ballot(in && reaches(start, b, unit, mul, add, div));
+    const int hit = reached ? 63 - __builtin_clzll(reached) : 0;
+    Sequence r = make_sequence(low + hit, __builtin_amdgcn_readlane(start, hit), __builtin_amdgcn_readlane(end, hit),
+            __builtin_amdgcn_readlane(length, hit));
+    r.base = unit_base(r.row0, r.b, mul, add, div);
     return r;
 }
 

@@ -18,8 +18,9 @@ void check(const bool ok, const char *what) {
 int search(const std::vector<int> &starts, const int batch, const int tokens, const uint32_t unit, const uint32_t mul, const uint32_t add,
         const uint32_t div) {
     int low = 0, span = batch;
-    while (span > 1) {
-        const int step = rk::search_step(span);
+    for (bool last = false; !last;) {
+        last = span <= 64;
+        const int step = rk::search_step(span); // 1 in the last round
         int hit = 0;
         for (int lane = 0; lane < 64; ++lane) {
             const int b = low + lane * step;
