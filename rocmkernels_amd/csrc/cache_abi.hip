@@ -80,7 +80,7 @@ int attention_cache_forward(const void *q, rocmkernels_cache cache, rocmkernels_
     const int window = radius >= kPositionLimit ? -1 : radius;
     const rk::CacheForwardArgs a{q, view(cache), view(sequences), output, lse, query_heads, keys, window,
             flags & ROCMKERNELS_ATTENTION_CAUSAL, qs, os, dtype, workspace};
-    const rk::ForwardPlan plan = rk::plan_cache_forward(cache.width, a.seqs, cache.heads, query_heads, keys, window);
+    const rk::ForwardPlan plan = rk::plan_cache_forward(cache.width, a.seqs, cache.heads, query_heads, keys, window, a.causal != 0);
     if (plan.workspace > 0 && (!workspace || misaligned(workspace, 15) || workspace_bytes < plan.workspace)) return kInvalid;
     return rk::launch_cache_forward(cache.width, a, plan, stream);
 }
@@ -91,7 +91,7 @@ int attention_cache_workspace(rocmkernels_cache cache, rocmkernels_sequences seq
     const int keys = key_limit(cache, sequences, max_keys);
     if (keys < 0) return kInvalid;
     *bytes = sequences.tokens == 0 ? 0
-                                   : rk::plan_cache_forward(cache.width, view(sequences), cache.heads, query_heads, keys, -1)
+                                   : rk::plan_cache_forward(cache.width, view(sequences), cache.heads, query_heads, keys, -1, false)
                                              .workspace_most;
     return hipSuccess;
 }

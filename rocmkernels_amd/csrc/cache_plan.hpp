@@ -68,7 +68,7 @@ constexpr int kSmallRows = 32;  // sequences of up to this many flattened rows a
 constexpr int kLargeTile = 128; // rows of a large tile
 
 inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, const int heads, const int query_heads, const int max_keys,
-        const int radius) {
+        const int radius, const bool causal) {
     const int group = query_heads / heads;
     const long long flat = static_cast<long long>(s.tokens) * group;
     ForwardPlan p{};
@@ -76,12 +76,12 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
     auto cut = [&](ForwardPart &part, const long long workgroups, const int least_steps) {
         // The keys that a tile may see: all, or its window.
         long long span = max_keys;
-        if (radius >= 0) span = std::min(span, 2ll * radius + 1 + (part.rows + group - 1) / group + kStep);
+        if (radius >= 0) span = std::min(span, (causal ? 1ll : 2ll) * radius + 1 + (part.rows + group - 1) / group + kStep);
         const long long steps = (span + kStep - 1) / kStep;
         const long long pairs = static_cast<long long>(part.units) * heads;
         const long long wanted = (workgroups + pairs - 1) / std::max(pairs, 1ll);
         const long long chunks = std::min(wanted, std::max(1ll, steps / least_steps)); // grows with the keys and the window
-        part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks);
+        part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks + 3) / 4 * 4; // four waves take turns in a small tile
         part.chunks = static_cast<int>((steps + part.chunk_steps - 1) / part.chunk_steps);
         const size_t chunk_bytes = static_cast<size_t>(pairs) * part.rows * (width + 4) * sizeof(float);
         part.workspace = part.chunks > 1 ? chunk_bytes * part.chunks : 0;
@@ -104,7 +104,7 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         p.small.units = small_only ? static_cast<int>(row_units(flat, s.batch, 16)) : s.batch * p.small.direct;
         p.small.least = 1;
         p.small.most = small_only ? 0x7fffffff : kSmallRows;
-        cut(p.small, 2048, 8);
+        cut(p.small, 2048, 16);
     }
     p.workspace_most = most;
     return p;

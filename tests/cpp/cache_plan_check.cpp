@@ -72,9 +72,9 @@ int main() {
         // Plans.
         const rk::SequenceView s{nullptr, nullptr, nullptr, batch, tokens, 1, 1};
         const int heads = pick(1, 12), keys = pick(0, 2) ? pick(1, 5000) : pick(1, 200000), width = 32 << pick(0, 2);
-        const size_t whole = rk::plan_cache_forward(width, s, heads, heads * group, keys, -1).workspace_most;
+        const size_t whole = rk::plan_cache_forward(width, s, heads, heads * group, keys, -1, false).workspace_most;
         for (const int radius : {-1, 0, 1, 100, 777, 5000, 100000}) {
-            const rk::ForwardPlan p = rk::plan_cache_forward(width, s, heads, heads * group, keys, radius);
+            const rk::ForwardPlan p = rk::plan_cache_forward(width, s, heads, heads * group, keys, radius, round % 2 == 0);
             check(p.workspace <= whole, "a window needs more workspace than the whole");
             check(p.small.workspace + p.large.workspace == p.workspace, "parts of the workspace");
             for (const rk::ForwardPart *part : {&p.small, &p.large}) {
