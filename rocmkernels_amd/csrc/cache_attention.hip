@@ -565,12 +565,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         e.absent = static_cast<uint32_t>(__ballot(place < 0) >> (4 * turn)) & 15u;
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
-            // K: token x / (D / 16), 16 of its features; V: block x / D, feature x % D. Blocks that are not there read the cache's first.
-            const int x = threadIdx.x + n * kThreads, token = x / (D / 16), block = x / D;
-            const int64_t kb = max(__shfl(place, 4 * turn + min(token / 16, 3)), 0), vb = max(__shfl(place, 4 * turn + min(block, 3)), 0);
-            if (ALL || x < kStep * D / 16) {
-                raw_k[n] = *reinterpret_cast<const u32x4 *>(a.cache.keys + kb * (kBlockTokens * D) + (token % 16) * D + (x % (D / 16)) * 16);
-                raw_v[n] = *reinterpret_cast<const u32x4 *>(a.cache.values + vb * (kBlockTokens * D) + (x % D) * 16);
+            // K: token x / (D / 16), 16 of its features; V: block x / D, feature x % D, with x = thread + n * kThreads. From D = 64 on a
+            // wave's 64 chunks of either lie in one block, at D = 32 in two. Blocks that are not there read the cache's first.
+            constexpr int SHARE = D / 64; // waves that share a block
+            int64_t at;
+            if constexpr (D >= 64) at = max(__builtin_amdgcn_readlane(place, 4 * turn + wave / SHARE + n * (kWaves / SHARE)), 0);
+            else at = max(__shfl(place, 4 * turn + (2 * wave + h) % 4), 0);
+            if (ALL || wave < 2) {
+                const uint32_t token = (threadIdx.x / (D / 16)) % 16;
+                raw_k[n] = *reinterpret_cast<const u32x4 *>(a.cache.keys + at * (kBlockTokens * D) + (token * D + threadIdx.x % (D / 16) * 16));
+                raw_v[n] = *reinterpret_cast<const u32x4 *>(a.cache.values + at * (kBlockTokens * D) + threadIdx.x % D * 16);
             }
         }
     };
