@@ -339,10 +339,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             for (int u = 0; u < 2; ++u) {
                 float w[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[j] = exp2_fast(fmaf(sc[n][2 * u + j / 4][j % 4], c, -r));
-                    sum += w[j];
-                }
+                for (int j = 0; j < 8; ++j) w[j] = exp2_fast(fmaf(sc[n][2 * u + j / 4][j % 4], c, -r));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += w[j];
                 split_terms<TWO>(wh[u], wl[u], w);
             }
             l[n] = fmaf(sum, inverse, l[n]);
@@ -454,7 +453,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 // hold the tokens 16 u + 8 h .. + 7: one page's scales for eight scores, and the operand of V's block u as it lies in memory.
 // Staged layouts: K [8-feature chunk][token] and V [block][half][feature] of 16 bytes, so operand reads cover 512 contiguous bytes a
 // half-wave; a K chunk is padded by 16 * 128 / D bytes, which puts the writes of 16 neighbouring lanes on distinct banks.
-template<int T, int D, bool VEC>
+//
+// GROUPS: groups of a step's keys that share their scales, one where pages are multiples of 64 tokens, else a group for each block.
+template<int T, int D, bool VEC, int GROUPS>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_large_kernel(const CacheForwardArgs a,
         const ForwardPart part) {
     constexpr bool TWO = T == kFloat32;
@@ -615,15 +616,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         if (wave_rows <= 0 || key0 >= any_high || key0 + kStep <= any_low) return;
         const uint8_t *const k = staged[index & 1] + token_of_row * 16 + h * K_CHUNK;
         const uint8_t *const v = staged[index & 1] + K_BYTES + (h * D + col) * 16;
-        f32x16 sc[2];
-        sc[0] = sc[1] = f32x16{};
+        // LDS answers after several products' time, so operands are asked for well ahead: all of the first tile's K, then the second
+        // tile's as the first's are used, V's first block before the softmax, and each next block before the one at hand is weighed.
+        f32x16 sc[2] = {f32x16{}, f32x16{}};
+        f16x8 kx[KC], vx[2][DT];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) { // two independent chains
+        for (int c = 0; c < KC; ++c) kx[c] = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const f16x8 w = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK) + n * 512);
-                sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[c], sc[n], 0, 0, 0);
-                if constexpr (TWO) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[c], sc[n], 0, 0, 0);
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[c], qh[c], sc[n], 0, 0, 0);
+                if constexpr (TWO) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[c], ql[c], sc[n], 0, 0, 0);
+                if (n == 0) kx[c] = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK) + 512);
+                else if (c < DT) vx[0][c] = *reinterpret_cast<const f16x8 *>(v + 32 * c * 16);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         const bool full = key0 >= all_low && key0 + kStep <= all_high && e.absent == 0;
@@ -639,16 +647,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) any_nan |= nan_flags[index & 1][w] != 0;
         }
-        float c[4], candidate = -INFINITY;
+        constexpr int BLOCKS = 4 / GROUPS;
+        float c[GROUPS], ev[GROUPS], candidate = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < GROUPS; ++b) {
             c[b] = fmaxf(c2 * power(static_cast<int8_t>(e.exps[b])), 1.17549435e-38f); // > 0, so that hidden scores stay -inf
+            ev[b] = static_cast<float>(static_cast<int8_t>(e.exps[b] >> 8));
             float most = sc[b / 2][8 * (b % 2)];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[b / 2][8 * (b % 2) + j]);
+            for (int j = 1; j < 8 * BLOCKS; ++j) most = fmaxf(most, sc[(b * BLOCKS + j / 8) / 2][8 * ((b * BLOCKS + j / 8) % 2) + j % 8]);
             most *= c[b];
             m = fmaxf(m, most);
-            candidate = fmaxf(candidate, most + static_cast<float>(static_cast<int8_t>(e.exps[b] >> 8)));
+            candidate = fmaxf(candidate, most + ev[b]);
         }
         if (__ballot(candidate > M + kLazyRange)) {
             const float raised = halves_max(fmaxf(M, candidate));
@@ -659,25 +669,33 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             for (int d = 0; d < DT; ++d) acc[d] *= alpha;
         }
         const float reference = (M == -INFINITY ? 0.0f : M) - kWeightShift;
+        float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const int ev = static_cast<int8_t>(e.exps[b] >> 8);
-            const float rb = reference - static_cast<float>(ev);
-            float w[8], sum = 0.0f;
+            const int of = b / BLOCKS;
+            const float r = reference - ev[of];
+            if (b < 3) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = exp2_fast(fmaf(sc[b / 2][8 * (b % 2) + j], c[b], -rb));
-                sum += w[j];
+                for (int d = 0; d < DT; ++d) vx[(b + 1) % 2][d] = *reinterpret_cast<const f16x8 *>(v + (2 * (b + 1) * D + 32 * d) * 16);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            l = fmaf(sum, power(-ev), l);
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = exp2_fast(fmaf(sc[b / 2][8 * (b % 2) + j], c[of], -r));
             f16x8 wh, wl;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += w[j];
             split_terms<TWO>(wh, wl, w);
+            if (b % BLOCKS == BLOCKS - 1) {
+                l = fmaf(sum, power(-static_cast<int8_t>(e.exps[of] >> 8)), l);
+                sum = 0.0f;
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const f16x8 x = *reinterpret_cast<const f16x8 *>(v + (2 * b * D + 32 * d) * 16);
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, acc[d], 0, 0, 0);
-                if constexpr (TWO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, acc[d], 0, 0, 0);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[b % 2][d], wh, acc[d], 0, 0, 0);
+                if constexpr (TWO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[b % 2][d], wl, acc[d], 0, 0, 0);
             }
+            __asm__ volatile("" : "+v"(l), "+v"(sum)); // the sums are formed here, not sunk behind the step: that kept all weights alive
         }
         if (__builtin_expect(any_nan, 0)) {
             // Count the NaN values that each row sees with a product of ones (0x38 is 1.0 in e4m3); V's bytes are read again.
@@ -824,7 +842,12 @@ template<int T, int D, bool VEC>
 void launch(const CacheForwardArgs &a, const ForwardPlan &plan, hipStream_t stream) {
     if (plan.large.units > 0) {
         const uint32_t pairs = static_cast<uint32_t>(plan.large.units) * a.cache.heads;
-        hipLaunchKernelGGL((cache_attention_large_kernel<T, D, VEC>), dim3(pairs * plan.large.chunks), dim3(kThreads), 0, stream, a, plan.large);
+        if (a.cache.page_size % kStep == 0)
+            hipLaunchKernelGGL((cache_attention_large_kernel<T, D, VEC, 1>), dim3(pairs * plan.large.chunks), dim3(kThreads), 0, stream, a,
+                    plan.large);
+        else
+            hipLaunchKernelGGL((cache_attention_large_kernel<T, D, VEC, 4>), dim3(pairs * plan.large.chunks), dim3(kThreads), 0, stream, a,
+                    plan.large);
         if (plan.large.chunks > 1) launch_join<T, D, VEC>(a, plan.large, pairs, stream);
     }
     if (plan.small.units > 0) {
