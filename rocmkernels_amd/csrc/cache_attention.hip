@@ -137,45 +137,43 @@ __device__ __forceinline__ void split_terms(f16x8 &hi, f16x8 &lo, const float (&
     }
 }
 
-// NQ tiles of 16 rows a workgroup.
-template<int T, int D, int NQ, bool VEC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_kernel(const CacheForwardArgs a,
-        const ForwardPart part) {
+// A tile of 16 rows: each wave streams its own keys, and the four are merged through LDS.
+template<int D>
+constexpr int kSmallShared = kWaves * 16 * (D + 4) * 4 + kWaves * 16 * 4 * 4; // bytes
+
+template<int T, int D, bool VEC>
+__device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const ForwardPart &part, const uint32_t number, uint8_t *shared) {
     constexpr bool TWO = T == kFloat32;
     constexpr int KC = D / 32;                   // MFMAs of a score tile
     constexpr int KL = D >= 64 ? D / 64 : 1;     // loads of a K row tile
     constexpr int DT = D / 16;                   // output tiles
-    constexpr int ROWS = 16 * NQ;
-    constexpr int STRIDE = D + 4;
-    __shared__ float merged[kWaves][ROWS][STRIDE];
-    __shared__ float stats[kWaves][ROWS][4];
+    constexpr int ROWS = 16;
+    auto merged = reinterpret_cast<float(*)[ROWS][D + 4]>(shared);
+    auto stats = reinterpret_cast<float(*)[ROWS][4]>(shared + kWaves * ROWS * (D + 4) * 4);
 
     const int lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int heads = a.cache.heads, group = a.query_heads / heads;
-    const uint32_t slot = blockIdx.x, pair = slot / part.chunks;
-    const int chunk = static_cast<int>(slot - pair * part.chunks);
-    const uint32_t unit = pair / heads;
-    const int head = static_cast<int>(pair - unit * heads);
+    // First chunks first: every sequence has one, and the short ends of sequences come last, when the chip runs empty.
+    const uint32_t pairs = static_cast<uint32_t>(part.units) * heads, pair = number % pairs, unit = pair / heads;
+    const int chunk = static_cast<int>(number / pairs), head = static_cast<int>(pair - unit * heads);
+    const int64_t slot = static_cast<int64_t>(pair) * part.chunks + chunk;
 
     const Tile t = tile_of(a, part, unit, group);
     if (t.rows <= 0 || chunk >= max(t.chunks, 1)) return;
     const int step_begin = t.step0 + chunk * part.chunk_steps;
     const int step_end = t.step0 + min(t.steps, (chunk + 1) * part.chunk_steps);
 
-    // This lane's rows: q in operand order, the factor of its scores, and the keys it sees.
-    f16x8 qh[NQ][KC], ql[TWO ? NQ : 1][TWO ? KC : 1];
-    float c2[NQ];
-    int low[NQ], high[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int r = 16 * n + col;
-        const bool used = r < t.rows;
-        const int flat = t.row0 + (used ? r : 0), i = flat / group, query_head = head * group + (flat - i * group);
+    // This lane's row: q in operand order, the factor of its scores, and the keys it sees. Lanes past the last row repeat the first.
+    f16x8 qh[KC], ql[TWO ? KC : 1];
+    float c2;
+    int low, high;
+    {
+        const int flat = t.row0 + (col < t.rows ? col : 0), i = flat / group, query_head = head * group + (flat - i * group);
         const int64_t row = static_cast<int64_t>(t.s.row0 + i) * a.qs.token + static_cast<int64_t>(query_head) * a.qs.head;
         const int position = t.s.first + i;
-        low[n] = t.vis.low(position);
-        high[n] = t.vis.high(position);
+        low = t.vis.low(position);
+        high = t.vis.high(position);
         float x[KC][8];
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
@@ -196,27 +194,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             scale = power(14 - e);
             back = power(e - 14);
         }
-        c2[n] = back * (kLog2e / sqrtf(static_cast<float>(D)));
+        c2 = back * (kLog2e / sqrtf(static_cast<float>(D)));
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[k][j] *= scale;
-            split_terms<TWO>(qh[n][k], ql[TWO ? n : 0][TWO ? k : 0], x[k]);
+            split_terms<TWO>(qh[k], ql[TWO ? k : 0], x[k]);
         }
     }
     // Keys that every row sees: between the last row's first key and the first row's end.
     const int all_low = t.vis.low(t.s.first + (t.row0 + t.rows - 1) / group), all_high = t.vis.high(t.s.first + t.row0 / group);
 
-    float M[NQ], l[NQ], m[NQ];
-    f32x4 acc[NQ][DT];
+    float M = -INFINITY, l = 0.0f, m = -INFINITY;
+    f32x4 acc[DT];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        M[n] = -INFINITY;
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[n][d] = f32x4{};
-    }
+    for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
 
     // The 64 blocks of this wave's next 16 steps, one a lane: the block's place in the cache (-1: none) and its exponents.
     const int blocks = a.cache.page_size / kBlockTokens;
@@ -266,35 +258,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         const int exps = __shfl(exponents, 4 * turn + g);
         const int ek = static_cast<int16_t>(exps & 0xffff), ev = exps >> 16;
         const float fev = static_cast<float>(ev), inverse = power(-ev), kscale = power(ek);
-        f32x4 sc[NQ][4];
+        f32x4 sc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) sc[n][i] = f32x4{};
+            sc[i] = f32x4{};
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
                 const f16x8 w = widen(x.k[i][k / 2][2 * (k % 2)], x.k[i][k / 2][2 * (k % 2) + 1]);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    sc[n][i] = mfma_16(w, qh[n][k], sc[n][i]);
-                    if constexpr (TWO) sc[n][i] = mfma_16(w, ql[n][k], sc[n][i]);
-                }
+                sc[i] = mfma_16(w, qh[k], sc[i]);
+                if constexpr (TWO) sc[i] = mfma_16(w, ql[k], sc[i]);
             }
         }
         const int key0 = kStep * step, base = key0 + 16 * g;
         const bool full = key0 >= all_low && key0 + kStep <= all_high && ((absent >> (4 * turn)) & 15u) == 0;
-        uint32_t visible[NQ], held = 0;
+        uint32_t visible = 0, held = 0;
         bool any_nan = false;
         if (!full) {
             const bool here = !((absent >> (4 * turn + g)) & 1u);
+            visible = here ? bit_range(low - base, high - base - 1) & 0xffffu : 0u;
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                visible[n] = here ? bit_range(low[n] - base, high[n] - base - 1) & 0xffffu : 0u;
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[n][i][j] = (visible[n] >> (4 * i + j)) & 1u ? sc[n][i][j] : -INFINITY;
-                }
+                for (int j = 0; j < 4; ++j) sc[i][j] = (visible >> (4 * i + j)) & 1u ? sc[i][j] : -INFINITY;
             }
             // Bytes behind the sequence's end may hold anything, and 0 times NaN is no 0: NaN counts for the rows that see its key.
             held = here ? bit_range(0, t.vis.length - base - 1) & 0xffffu : 0u;
@@ -310,82 +295,69 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             }
             any_nan = __ballot(nans != 0) != 0;
         }
+        const float c = fmaxf(c2 * kscale, 1.17549435e-38f); // > 0, so that hidden scores stay -inf
+        float most = sc[0][0];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const float c = fmaxf(c2[n] * kscale, 1.17549435e-38f); // > 0, so that hidden scores stay -inf
-            float most = sc[n][0][0];
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, sc[i][j]);
+        }
+        most *= c;
+        m = fmaxf(m, most);
+        const float candidate = most + fev;
+        if (__ballot(candidate > M + kLazyRange)) {
+            float raised = fmaxf(M, candidate);
+            raised = fmaxf(raised, __shfl_xor(raised, 16));
+            raised = fmaxf(raised, __shfl_xor(raised, 32));
+            const float alpha = M == raised ? 1.0f : exp2_fast(M - raised);
+            M = raised;
+            l *= alpha;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) most = fmaxf(most, sc[n][i][j]);
-            }
-            most *= c;
-            m[n] = fmaxf(m[n], most);
-            const float candidate = most + fev;
-            if (__ballot(candidate > M[n] + kLazyRange)) {
-                float raised = fmaxf(M[n], candidate);
-                raised = fmaxf(raised, __shfl_xor(raised, 16));
-                raised = fmaxf(raised, __shfl_xor(raised, 32));
-                const float alpha = M[n] == raised ? 1.0f : exp2_fast(M[n] - raised);
-                M[n] = raised;
-                l[n] *= alpha;
+            for (int d = 0; d < DT; ++d) acc[d] *= alpha;
+        }
+        const float r = (M == -INFINITY ? 0.0f : M) - fev - kWeightShift;
+        float sum = 0.0f;
+        f16x8 wh[2], wl[2];
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[n][d] *= alpha;
-            }
-            const float r = (M[n] == -INFINITY ? 0.0f : M[n]) - fev - kWeightShift;
-            float sum = 0.0f;
-            f16x8 wh[2], wl[2];
+        for (int u = 0; u < 2; ++u) {
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = exp2_fast(fmaf(sc[2 * u + j / 4][j % 4], c, -r));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += w[j];
+            split_terms<TWO>(wh[u], wl[u], w);
+        }
+        l = fmaf(sum, inverse, l);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = exp2_fast(fmaf(sc[n][2 * u + j / 4][j % 4], c, -r));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += w[j];
-                split_terms<TWO>(wh[u], wl[u], w);
-            }
-            l[n] = fmaf(sum, inverse, l[n]);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const f16x8 v = widen(x.v[d][2 * u], x.v[d][2 * u + 1]);
-                    acc[n][d] = mfma_16(v, wh[u], acc[n][d]);
-                    if constexpr (TWO) acc[n][d] = mfma_16(v, wl[u], acc[n][d]);
-                }
+                const f16x8 v = widen(x.v[d][2 * u], x.v[d][2 * u + 1]);
+                acc[d] = mfma_16(v, wh[u], acc[d]);
+                if constexpr (TWO) acc[d] = mfma_16(v, wl[u], acc[d]);
             }
         }
         if (__builtin_expect(any_nan, 0)) {
             // Count the NaN values that each row sees with a product of ones (0x38 is 1.0 in e4m3); V's bytes are read again.
             const int64_t vb = max(__shfl(place, 4 * turn + g), 0);
             const uint8_t *const v = a.cache.values + vb * (kBlockTokens * D) + col * 16;
-#pragma unroll 1
-            for (int n = 0; n < NQ; ++n) {
-                f16x8 sees[2];
+            f16x8 sees[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t bits = visible[0];
-                        if constexpr (NQ > 1) bits = n == 0 ? visible[0] : visible[NQ - 1];
-                        sees[u][j] = static_cast<_Float16>((bits >> (8 * u + j)) & 1u ? 1.0f : 0.0f);
-                    }
-                }
+                for (int j = 0; j < 8; ++j) sees[u][j] = static_cast<_Float16>((visible >> (8 * u + j)) & 1u ? 1.0f : 0.0f);
+            }
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const u32x4 y = *reinterpret_cast<const u32x4 *>(v + d * 256);
-                    f32x4 hits{};
+            for (int d = 0; d < DT; ++d) {
+                const u32x4 y = *reinterpret_cast<const u32x4 *>(v + d * 256);
+                f32x4 hits{};
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        hits = mfma_16(widen(nan_bytes(y[2 * u] & byte_mask(held >> (8 * u))) & 0x38383838u,
-                                               nan_bytes(y[2 * u + 1] & byte_mask(held >> (8 * u + 4))) & 0x38383838u),
-                                sees[u], hits);
+                for (int u = 0; u < 2; ++u)
+                    hits = mfma_16(widen(nan_bytes(y[2 * u] & byte_mask(held >> (8 * u))) & 0x38383838u,
+                                           nan_bytes(y[2 * u + 1] & byte_mask(held >> (8 * u + 4))) & 0x38383838u),
+                            sees[u], hits);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                        for (int k = 0; k < NQ; ++k) acc[k][d][j] = k == n && hits[j] > 0.0f ? NAN : acc[k][d][j];
-                    }
-                }
+                for (int j = 0; j < 4; ++j) acc[d][j] = hits[j] > 0.0f ? NAN : acc[d][j];
             }
         }
     };
@@ -401,21 +373,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     }
 
     // Merge: each wave's sums over the lanes of a column, then the four waves.
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        l[n] += __shfl_xor(l[n], 16);
-        l[n] += __shfl_xor(l[n], 32);
-        m[n] = fmaxf(m[n], __shfl_xor(m[n], 16));
-        m[n] = fmaxf(m[n], __shfl_xor(m[n], 32));
-        const int r = 16 * n + col;
-        if (g == 0) {
-            stats[wave][r][0] = M[n];
-            stats[wave][r][1] = l[n];
-            stats[wave][r][2] = m[n];
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(&merged[wave][r][16 * d + 4 * g]) = acc[n][d];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    if (g == 0) {
+        stats[wave][col][0] = M;
+        stats[wave][col][1] = l;
+        stats[wave][col][2] = m;
     }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(&merged[wave][col][16 * d + 4 * g]) = acc[d];
     __syncthreads();
     constexpr int SPAN = 8;
     for (int i = threadIdx.x; i < ROWS * (D / SPAN); i += kThreads) {
@@ -455,18 +423,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 // half-wave; a K chunk is padded by 16 * 128 / D bytes, which puts the writes of 16 neighbouring lanes on distinct banks.
 //
 // GROUPS: groups of a step's keys that share their scales, one where pages are multiples of 64 tokens, else a group for each block.
+template<int D>
+constexpr int kChunkBytes = kStep * 16 + 16 * 128 / D; // a staged 8-feature chunk of K
+template<int D>
+constexpr int kLargeShared = 2 * (D / 8 * kChunkBytes<D> + kStep * D * 2) + 2 * kWaves * 4; // bytes
+
 template<int T, int D, bool VEC, int GROUPS>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_large_kernel(const CacheForwardArgs a,
-        const ForwardPart part) {
+__device__ __forceinline__ void large_tile(const CacheForwardArgs &a, const ForwardPart &part, const uint32_t number, uint8_t *shared) {
     constexpr bool TWO = T == kFloat32;
     constexpr int KC = D / 16;                       // MFMAs of a 32-key score tile
     constexpr int DT = D / 32;                       // output tiles
-    constexpr int K_CHUNK = kStep * 16 + 16 * 128 / D;
+    constexpr int K_CHUNK = kChunkBytes<D>;
     constexpr int K_BYTES = D / 8 * K_CHUNK, V_BYTES = kStep * D * 2;
     constexpr int LOADS = (kStep * D / 16 + kThreads - 1) / kThreads; // 16-byte loads of K, and of V, of a thread
     constexpr bool ALL = kStep * D / 16 >= kThreads; // D = 32: half the threads load
-    __shared__ __align__(16) uint8_t staged[2][K_BYTES + V_BYTES];
-    __shared__ int nan_flags[2][kWaves];
+    auto staged = reinterpret_cast<uint8_t(*)[K_BYTES + V_BYTES]>(shared);
+    auto nan_flags = reinterpret_cast<int(*)[kWaves]>(shared + 2 * (K_BYTES + V_BYTES));
 
     const int lane = threadIdx.x & (kWave - 1), col = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -474,7 +446,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     // Workgroups go round the 8 XCDs: give each XCD whole heads, whose keys then stay in its L2, and of a head the last tiles
     // (under a causal mask the longest) first.
     const uint32_t pairs = static_cast<uint32_t>(part.units) * heads, total = pairs * part.chunks;
-    const uint32_t xcd = blockIdx.x % 8, place_in_order = xcd * (total / 8) + min(xcd, total % 8) + blockIdx.x / 8;
+    const uint32_t xcd = number % 8, place_in_order = xcd * (total / 8) + min(xcd, total % 8) + number / 8;
     const int head = static_cast<int>(place_in_order / (part.units * part.chunks));
     const uint32_t rest = place_in_order - static_cast<uint32_t>(head) * part.units * part.chunks;
     const uint32_t unit = part.units - 1 - rest / part.chunks;
@@ -619,7 +591,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         // LDS answers after several products' time, so operands are asked for well ahead: all of the first tile's K, then the second
         // tile's as the first's are used, V's first block before the softmax, and each next block before the one at hand is weighed.
         f32x16 sc[2] = {f32x16{}, f32x16{}};
-        f16x8 kx[KC], vx[2][DT];
+        constexpr bool AHEAD = !(TWO && D == 128); // V's operands, where registers allow
+        f16x8 kx[KC], vx[AHEAD ? 2 : 1][DT];
 #pragma unroll
         for (int c = 0; c < KC; ++c) kx[c] = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK));
         __builtin_amdgcn_sched_barrier(0);
@@ -630,7 +603,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
                 sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[c], qh[c], sc[n], 0, 0, 0);
                 if constexpr (TWO) sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[c], ql[c], sc[n], 0, 0, 0);
                 if (n == 0) kx[c] = *reinterpret_cast<const f16x8 *>(k + c * (2 * K_CHUNK) + 512);
-                else if (c < DT) vx[0][c] = *reinterpret_cast<const f16x8 *>(v + 32 * c * 16);
+                else if (AHEAD && c < DT) vx[0][c] = *reinterpret_cast<const f16x8 *>(v + 32 * c * 16);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -674,9 +647,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         for (int b = 0; b < 4; ++b) {
             const int of = b / BLOCKS;
             const float r = reference - ev[of];
-            if (b < 3) {
+            if (AHEAD && b < 3) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) vx[(b + 1) % 2][d] = *reinterpret_cast<const f16x8 *>(v + (2 * (b + 1) * D + 32 * d) * 16);
+                for (int d = 0; d < DT; ++d) vx[AHEAD ? (b + 1) % 2 : 0][d] = *reinterpret_cast<const f16x8 *>(v + (2 * (b + 1) * D + 32 * d) * 16);
                 __builtin_amdgcn_sched_barrier(0);
             }
             float w[8];
@@ -692,8 +665,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[b % 2][d], wh, acc[d], 0, 0, 0);
-                if constexpr (TWO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[b % 2][d], wl, acc[d], 0, 0, 0);
+                const f16x8 x = AHEAD ? vx[AHEAD ? b % 2 : 0][d] : *reinterpret_cast<const f16x8 *>(v + (2 * b * D + 32 * d) * 16);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wh, acc[d], 0, 0, 0);
+                if constexpr (TWO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, wl, acc[d], 0, 0, 0);
             }
             __asm__ volatile("" : "+v"(l), "+v"(sum)); // the sums are formed here, not sunk behind the step: that kept all weights alive
         }
@@ -760,10 +734,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     }
 }
 
+template<int T, int D, bool VEC>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_small_kernel(
+        const CacheForwardArgs a,
+        const ForwardPart part) {
+    __shared__ __align__(16) uint8_t shared[kSmallShared<D>];
+    small_tile<T, D, VEC>(a, part, blockIdx.x, shared);
+}
+
+// Large tiles and, in the workgroups behind theirs, small ones: in a batch that mixes prompts with single tokens the matrix
+// work of the first and the memory traffic of the second run side by side.
+template<int T, int D, bool VEC, int GROUPS>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_kernel(const CacheForwardArgs a,
+        const ForwardPart large, const ForwardPart small, const uint32_t large_groups) {
+    __shared__ __align__(16) uint8_t shared[std::max(kSmallShared<D>, kLargeShared<D>)];
+    if (blockIdx.x < large_groups) large_tile<T, D, VEC, GROUPS>(a, large, blockIdx.x, shared);
+    else small_tile<T, D, VEC>(a, small, blockIdx.x - large_groups, shared);
+}
+
 // Joins the chunks of a tile, in an order that their number fixes. D / 4 lanes hold a row's features; the other lanes of a wave,
 // and for many chunks the other waves of the workgroup, take chunks of their own with a running reference and are merged at the end.
-// WAVES: waves that share a row; with one, a wave joins kJoinRows / 4 rows in turn.
-constexpr int kJoinRows = 16;
+constexpr int kJoinRows = 16;      // rows of a workgroup whose waves join a row each,
+constexpr int kJoinTogether = 8;   // up to this many chunks; with more the four waves share one row
 
 struct Joined {
     float reference = -INFINITY, most = -INFINITY, sum = 0.0f, o[4] = {};
@@ -779,23 +771,32 @@ struct Joined {
     }
 };
 
-template<int T, int D, bool VEC, int WAVES>
-__global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForwardArgs a, const ForwardPart part) {
+inline int join_rows(const ForwardPart &part) { return part.chunks > kJoinTogether ? 1 : kJoinRows; }
+inline uint32_t join_groups(const ForwardPart &part, const int heads) {
+    return part.chunks > 1 ? static_cast<uint32_t>(part.units) * heads * (part.rows / join_rows(part)) : 0;
+}
+
+template<int T, int D, bool VEC>
+__global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForwardArgs a, const ForwardPart large, const ForwardPart small,
+        const uint32_t large_groups) {
     constexpr int LANES = D / 4, SIDE = kWave / LANES; // chunks side by side in a wave
-    constexpr int ROWS = WAVES == 1 ? kJoinRows : 1;   // rows of a workgroup
     __shared__ float merged[kWaves][4 * LANES + 4];
+    const bool of_large = blockIdx.x < large_groups;
+    const ForwardPart part = of_large ? large : small;
+    const uint32_t number = of_large ? blockIdx.x : blockIdx.x - large_groups;
+    const int share = part.chunks > kJoinTogether ? kWaves : 1, rows = share > 1 ? 1 : kJoinRows; // waves of a row, rows of a workgroup
     const int heads = a.cache.heads, group = a.query_heads / heads;
-    const uint32_t row_groups = part.rows / ROWS, pair = blockIdx.x / row_groups, unit = pair / heads;
+    const uint32_t row_groups = part.rows / rows, pair = number / row_groups, unit = pair / heads;
     const int head = static_cast<int>(pair - unit * heads);
     const Tile t = tile_of(a, part, unit, group);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
-    const int first_row = static_cast<int>(blockIdx.x - pair * row_groups) * ROWS, f = 4 * (lane % LANES);
+    const int first_row = static_cast<int>(number - pair * row_groups) * rows, f = 4 * (lane % LANES);
     const int64_t slot = static_cast<int64_t>(pair) * part.chunks;
     if (t.chunks <= 1 || first_row >= t.rows) return;
-    for (int r = first_row + (WAVES == 1 ? wave : 0); r < min(first_row + ROWS, t.rows); r += kWaves) {
+    for (int r = first_row + (share > 1 ? 0 : wave); r < min(first_row + rows, t.rows); r += kWaves) {
         Joined row;
 #pragma unroll 4
-        for (int c = (WAVES == 1 ? 0 : wave * SIDE) + lane / LANES; c < t.chunks; c += WAVES * SIDE) {
+        for (int c = (share > 1 ? wave * SIDE : 0) + lane / LANES; c < t.chunks; c += share * SIDE) {
             const Partial p = partial_of<D>(a, part, slot + c, r);
             const f32x4 s = *reinterpret_cast<const f32x4 *>(p.stats), y = *reinterpret_cast<const f32x4 *>(p.acc + f);
             const float x[4] = {y[0], y[1], y[2], y[3]};
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForward
             for (int j = 0; j < 4; ++j) x[j] = __shfl_xor(row.o[j], m);
             row.add(__shfl_xor(row.reference, m), __shfl_xor(row.most, m), __shfl_xor(row.sum, m), x);
         }
-        if constexpr (WAVES > 1) {
+        if (share > 1) { // one row a workgroup: all waves are here
             if (lane < LANES) {
                 *reinterpret_cast<f32x4 *>(&merged[wave][f]) = f32x4{row.o[0], row.o[1], row.o[2], row.o[3]};
                 if (f == 0) *reinterpret_cast<f32x4 *>(&merged[wave][4 * LANES]) = f32x4{row.reference, row.most, row.sum, 0.0f};
@@ -816,7 +817,7 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForward
             __syncthreads();
             if (wave != 0) return;
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) {
+            for (int w = 1; w < kWaves; ++w) {
                 const f32x4 s = *reinterpret_cast<const f32x4 *>(&merged[w][4 * LANES]), y = *reinterpret_cast<const f32x4 *>(&merged[w][f]);
                 const float x[4] = {y[0], y[1], y[2], y[3]};
                 row.add(s[0], s[1], s[2], x);
@@ -829,35 +830,23 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForward
     }
 }
 
-template<int T, int D, bool VEC>
-void launch_join(const CacheForwardArgs &a, const ForwardPart &part, const uint32_t pairs, hipStream_t stream) {
-    // Many chunks: the waves of a workgroup share a row.
-    if (part.chunks > 8)
-        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, kWaves>), dim3(pairs * part.rows), dim3(kThreads), 0, stream, a, part);
-    else
-        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC, 1>), dim3(pairs * (part.rows / kJoinRows)), dim3(kThreads), 0, stream, a, part);
-}
+uint32_t attention_groups(const ForwardPart &part, const int heads) { return static_cast<uint32_t>(part.units) * heads * part.chunks; }
 
 template<int T, int D, bool VEC>
 void launch(const CacheForwardArgs &a, const ForwardPlan &plan, hipStream_t stream) {
-    if (plan.large.units > 0) {
-        const uint32_t pairs = static_cast<uint32_t>(plan.large.units) * a.cache.heads;
-        if (a.cache.page_size % kStep == 0)
-            hipLaunchKernelGGL((cache_attention_large_kernel<T, D, VEC, 1>), dim3(pairs * plan.large.chunks), dim3(kThreads), 0, stream, a,
-                    plan.large);
-        else
-            hipLaunchKernelGGL((cache_attention_large_kernel<T, D, VEC, 4>), dim3(pairs * plan.large.chunks), dim3(kThreads), 0, stream, a,
-                    plan.large);
-        if (plan.large.chunks > 1) launch_join<T, D, VEC>(a, plan.large, pairs, stream);
-    }
-    if (plan.small.units > 0) {
-        const uint32_t pairs = static_cast<uint32_t>(plan.small.units) * a.cache.heads;
-        if (plan.small.rows == 16)
-            hipLaunchKernelGGL((cache_attention_kernel<T, D, 1, VEC>), dim3(pairs * plan.small.chunks), dim3(kThreads), 0, stream, a, plan.small);
-        else
-            hipLaunchKernelGGL((cache_attention_kernel<T, D, 2, VEC>), dim3(pairs * plan.small.chunks), dim3(kThreads), 0, stream, a, plan.small);
-        if (plan.small.chunks > 1) launch_join<T, D, VEC>(a, plan.small, pairs, stream);
-    }
+    const int heads = a.cache.heads;
+    const uint32_t large = attention_groups(plan.large, heads), small = attention_groups(plan.small, heads);
+    if (large == 0)
+        hipLaunchKernelGGL((cache_attention_small_kernel<T, D, VEC>), dim3(small), dim3(kThreads), 0, stream, a, plan.small);
+    else if (a.cache.page_size % kStep == 0)
+        hipLaunchKernelGGL((cache_attention_kernel<T, D, VEC, 1>), dim3(large + small), dim3(kThreads), 0, stream, a, plan.large, plan.small,
+                large);
+    else
+        hipLaunchKernelGGL((cache_attention_kernel<T, D, VEC, 4>), dim3(large + small), dim3(kThreads), 0, stream, a, plan.large, plan.small,
+                large);
+    const uint32_t large_joins = join_groups(plan.large, heads), joins = large_joins + join_groups(plan.small, heads);
+    if (joins > 0)
+        hipLaunchKernelGGL((cache_join_kernel<T, D, VEC>), dim3(joins), dim3(kThreads), 0, stream, a, plan.large, plan.small, large_joins);
 }
 
 template<int T, int D>
@@ -876,9 +865,10 @@ void dispatch(const int width, const CacheForwardArgs &a, const ForwardPlan &pla
 } // namespace
 
 hipError_t launch_cache_forward(const int width, const CacheForwardArgs &a, const ForwardPlan &plan, hipStream_t stream) {
-    for (const ForwardPart *part : {&plan.small, &plan.large}) // threads of a launch, of the kernel and of the join
-        if (static_cast<long long>(part->units) * a.cache.heads * std::max(part->chunks, part->rows) >= (1ll << 32) / kThreads)
-            return hipErrorInvalidValue;
+    long long groups = 0; // of the kernel, or of the join if that has more
+    for (const ForwardPart *part : {&plan.small, &plan.large})
+        groups += static_cast<long long>(part->units) * a.cache.heads * std::max(part->chunks, part->chunks > 1 ? part->rows / join_rows(*part) : 1);
+    if (groups >= (1ll << 32) / kThreads) return hipErrorInvalidValue; // threads of a launch
     const int unit = a.dtype == kFloat32 ? 4 : 8;
     auto fits = [&](const void *p, const rocmkernels_strides &s) {
         return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (s.head % unit) == 0 && (s.token % unit) == 0;

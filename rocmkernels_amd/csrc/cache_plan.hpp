@@ -73,13 +73,14 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
     const long long flat = static_cast<long long>(s.tokens) * group;
     ForwardPlan p{};
     size_t most = 0;
-    auto cut = [&](ForwardPart &part, const long long workgroups, const int least_steps) {
+    // `tiles`: about how many of the units have rows, which the division over sequences leaves open.
+    auto cut = [&](ForwardPart &part, const long long tiles, const long long workgroups, const int least_steps) {
         // The keys that a tile may see: all, or its window.
         long long span = max_keys;
         if (radius >= 0) span = std::min(span, (causal ? 1ll : 2ll) * radius + 1 + (part.rows + group - 1) / group + kStep);
         const long long steps = (span + kStep - 1) / kStep;
         const long long pairs = static_cast<long long>(part.units) * heads;
-        const long long wanted = (workgroups + pairs - 1) / std::max(pairs, 1ll);
+        const long long filled = std::max(tiles * heads, 1ll), wanted = std::max((workgroups + filled / 2) / filled, 1ll);
         const long long chunks = std::min(wanted, std::max(1ll, steps / least_steps)); // grows with the keys and the window
         part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks + 3) / 4 * 4; // four waves take turns in a small tile
         part.chunks = static_cast<int>((steps + part.chunk_steps - 1) / part.chunk_steps);
@@ -96,7 +97,7 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         p.large.units = static_cast<int>(row_units(flat, s.batch, kLargeTile));
         p.large.least = s.batch > 1 ? kSmallRows + 1 : 1;
         p.large.most = 0x7fffffff;
-        cut(p.large, 512, 8);
+        cut(p.large, flat / kLargeTile, 512, 8);
     }
     if (small_only || s.batch > 1) {
         p.small.rows = 16;
@@ -104,7 +105,7 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         p.small.units = small_only ? static_cast<int>(row_units(flat, s.batch, 16)) : s.batch * p.small.direct;
         p.small.least = 1;
         p.small.most = small_only ? 0x7fffffff : kSmallRows;
-        cut(p.small, 2048, 16);
+        cut(p.small, small_only ? std::max(flat / 16, static_cast<long long>(std::min(s.batch, s.tokens))) : s.batch, 2048, 16);
     }
     p.workspace_most = most;
     return p;
