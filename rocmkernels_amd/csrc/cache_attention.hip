@@ -127,21 +127,31 @@ __device__ __forceinline__ Partial partial_of(const CacheForwardArgs &a, const F
     return {base + r * D, base + slots * part.rows * D + r * 4};
 }
 
-// The two terms of 8 values that are already scaled into fp16's range.
+// The two terms of 8 values that are already scaled into fp16's range: a pair is rounded by one packed conversion, and what is left
+// of each value by one mixed-precision FMA that reads the fp16 term and writes fp16 (the empty asm keeps the compiler from
+// taking the pair apart again).
 template<bool TWO>
 __device__ __forceinline__ void split_terms(f16x8 &hi, f16x8 &lo, const float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi[i] = static_cast<_Float16>(x[i]);
-        if constexpr (TWO) lo[i] = static_cast<_Float16>(x[i] - static_cast<float>(hi[i]));
+    for (int i = 0; i < 8; i += 2) {
+        f16x2 pair{static_cast<_Float16>(x[i]), static_cast<_Float16>(x[i + 1])};
+        if constexpr (TWO) {
+            uint32_t bits = __builtin_bit_cast(uint32_t, pair);
+            __asm__("" : "+v"(bits));
+            pair = __builtin_bit_cast(f16x2, bits);
+            lo[i] = static_cast<_Float16>(fmaf(x[i], 1.0f, -static_cast<float>(pair[0])));
+            lo[i + 1] = static_cast<_Float16>(fmaf(x[i + 1], 1.0f, -static_cast<float>(pair[1])));
+        }
+        hi[i] = pair[0];
+        hi[i + 1] = pair[1];
     }
 }
 
-// A tile of 16 rows: each wave streams its own keys, and the four are merged through LDS.
-template<int D>
-constexpr int kSmallShared = kWaves * 16 * (D + 4) * 4 + kWaves * 16 * 4 * 4; // bytes
+// A tile of 16 rows: each of the WAVES waves of the workgroup streams keys of its own, and they are merged through LDS.
+template<int D, int WAVES>
+constexpr int kSmallShared = WAVES * 16 * (D + 4) * 4 + WAVES * 16 * 4 * 4; // bytes
 
-template<int T, int D, bool VEC>
+template<int T, int D, bool VEC, int WAVES>
 __device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const ForwardPart &part, const uint32_t number, uint8_t *shared) {
     constexpr bool TWO = T == kFloat32;
     constexpr int KC = D / 32;                   // MFMAs of a score tile
@@ -149,7 +159,7 @@ __device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const Forw
     constexpr int DT = D / 16;                   // output tiles
     constexpr int ROWS = 16;
     auto merged = reinterpret_cast<float(*)[ROWS][D + 4]>(shared);
-    auto stats = reinterpret_cast<float(*)[ROWS][4]>(shared + kWaves * ROWS * (D + 4) * 4);
+    auto stats = reinterpret_cast<float(*)[ROWS][4]>(shared + WAVES * ROWS * (D + 4) * 4);
 
     const int lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -215,7 +225,7 @@ __device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const Forw
     int place = -1, exponents = 0;
     uint64_t absent = 0;
     auto look_up = [&](const int step) __attribute__((always_inline)) {
-        const int s = step + kWaves * (lane / 4), position = kStep * s + kBlockTokens * (lane % 4);
+        const int s = step + WAVES * (lane / 4), position = kStep * s + kBlockTokens * (lane % 4);
         place = -1;
         exponents = 0;
         if (s < step_end && position < t.vis.length) {
@@ -363,16 +373,16 @@ __device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const Forw
     };
 
     const int steps = step_end - step_begin - wave;
-    const int mine = steps > 0 ? (steps + kWaves - 1) / kWaves : 0;
+    const int mine = steps > 0 ? (steps + WAVES - 1) / WAVES : 0;
     for (int i = 0; i < mine; ++i) {
-        const int step = step_begin + wave + kWaves * i, turn = i % 16;
+        const int step = step_begin + wave + WAVES * i, turn = i % 16;
         if (turn == 0) look_up(step);
         Keys x;
         load_keys(x, turn);
         compute(x, turn, step);
     }
 
-    // Merge: each wave's sums over the lanes of a column, then the four waves.
+    // Merge: each wave's sums over the lanes of a column, then the waves.
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     m = fmaxf(m, __shfl_xor(m, 16));
@@ -386,17 +396,17 @@ __device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const Forw
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(&merged[wave][col][16 * d + 4 * g]) = acc[d];
     __syncthreads();
     constexpr int SPAN = 8;
-    for (int i = threadIdx.x; i < ROWS * (D / SPAN); i += kThreads) {
+    for (int i = threadIdx.x; i < ROWS * (D / SPAN); i += WAVES * kWave) {
         const int r = i / (D / SPAN), f = i % (D / SPAN) * SPAN;
         if (r >= t.rows) continue;
         float reference = -INFINITY, most = -INFINITY, sum = 0.0f, o[SPAN] = {};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             reference = fmaxf(reference, stats[w][r][0]);
             most = fmaxf(most, stats[w][r][2]);
         }
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float alpha = stats[w][r][0] == reference ? 1.0f : exp2_fast(stats[w][r][0] - reference);
             sum = fmaf(stats[w][r][1], alpha, sum);
 #pragma unroll
@@ -734,12 +744,11 @@ __device__ __forceinline__ void large_tile(const CacheForwardArgs &a, const Forw
     }
 }
 
-template<int T, int D, bool VEC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_small_kernel(
-        const CacheForwardArgs a,
-        const ForwardPart part) {
-    __shared__ __align__(16) uint8_t shared[kSmallShared<D>];
-    small_tile<T, D, VEC>(a, part, blockIdx.x, shared);
+template<int T, int D, bool VEC, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) __attribute__((amdgpu_waves_per_eu(WAVES > 8 ? 4 : 2))) void cache_attention_small_kernel(
+        const CacheForwardArgs a, const ForwardPart part) {
+    __shared__ __align__(16) uint8_t shared[kSmallShared<D, WAVES>];
+    small_tile<T, D, VEC, WAVES>(a, part, blockIdx.x, shared);
 }
 
 // Large tiles and, in the workgroups behind theirs, small ones: in a batch that mixes prompts with single tokens the matrix
@@ -747,9 +756,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 template<int T, int D, bool VEC, int GROUPS>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void cache_attention_kernel(const CacheForwardArgs a,
         const ForwardPart large, const ForwardPart small, const uint32_t large_groups) {
-    __shared__ __align__(16) uint8_t shared[std::max(kSmallShared<D>, kLargeShared<D>)];
+    __shared__ __align__(16) uint8_t shared[std::max(kSmallShared<D, kWaves>, kLargeShared<D>)];
     if (blockIdx.x < large_groups) large_tile<T, D, VEC, GROUPS>(a, large, blockIdx.x, shared);
-    else small_tile<T, D, VEC>(a, small, blockIdx.x - large_groups, shared);
+    else small_tile<T, D, VEC, kWaves>(a, small, blockIdx.x - large_groups, shared);
 }
 
 // Joins the chunks of a tile, in an order that their number fixes. D / 4 lanes hold a row's features; the other lanes of a wave,
@@ -793,15 +802,17 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForward
     const int first_row = static_cast<int>(number - pair * row_groups) * rows, f = 4 * (lane % LANES);
     const int64_t slot = static_cast<int64_t>(pair) * part.chunks;
     if (t.chunks <= 1 || first_row >= t.rows) return;
-    for (int r = first_row + (share > 1 ? 0 : wave); r < min(first_row + rows, t.rows); r += kWaves) {
-        Joined row;
+    // Lanes side by side hold different chunks of a row.
+    auto gather = [&](Joined &row, const int r, const int first, const int stride) __attribute__((always_inline)) {
 #pragma unroll 4
-        for (int c = (share > 1 ? wave * SIDE : 0) + lane / LANES; c < t.chunks; c += share * SIDE) {
+        for (int c = first + lane / LANES; c < t.chunks; c += stride) {
             const Partial p = partial_of<D>(a, part, slot + c, r);
             const f32x4 s = *reinterpret_cast<const f32x4 *>(p.stats), y = *reinterpret_cast<const f32x4 *>(p.acc + f);
             const float x[4] = {y[0], y[1], y[2], y[3]};
             row.add(s[0], s[2], s[1], x);
         }
+    };
+    auto across = [&](Joined &row) __attribute__((always_inline)) {
 #pragma unroll
         for (int m = LANES; m < kWave; m <<= 1) {
             float x[4];
@@ -809,23 +820,37 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(const CacheForward
             for (int j = 0; j < 4; ++j) x[j] = __shfl_xor(row.o[j], m);
             row.add(__shfl_xor(row.reference, m), __shfl_xor(row.most, m), __shfl_xor(row.sum, m), x);
         }
-        if (share > 1) { // one row a workgroup: all waves are here
-            if (lane < LANES) {
-                *reinterpret_cast<f32x4 *>(&merged[wave][f]) = f32x4{row.o[0], row.o[1], row.o[2], row.o[3]};
-                if (f == 0) *reinterpret_cast<f32x4 *>(&merged[wave][4 * LANES]) = f32x4{row.reference, row.most, row.sum, 0.0f};
-            }
-            __syncthreads();
-            if (wave != 0) return;
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) {
-                const f32x4 s = *reinterpret_cast<const f32x4 *>(&merged[w][4 * LANES]), y = *reinterpret_cast<const f32x4 *>(&merged[w][f]);
-                const float x[4] = {y[0], y[1], y[2], y[3]};
-                row.add(s[0], s[1], s[2], x);
-            }
-        }
+    };
+    auto finish = [&](const Joined &row, const int r) __attribute__((always_inline)) {
+        if (lane >= LANES || r >= t.rows) return;
+        const int flat = t.row0 + r, token = flat / group;
+        finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, row.o, row.sum, row.reference, row.most, f == 0);
+    };
+    if (share > 1) {
+        Joined row;
+        gather(row, first_row, wave * SIDE, kWaves * SIDE);
+        across(row);
         if (lane < LANES) {
-            const int flat = t.row0 + r, token = flat / group;
-            finish_row<T, VEC>(a, t.s.row0 + token, head * group + flat - token * group, f, row.o, row.sum, row.reference, row.most, f == 0);
+            *reinterpret_cast<f32x4 *>(&merged[wave][f]) = f32x4{row.o[0], row.o[1], row.o[2], row.o[3]};
+            if (f == 0) *reinterpret_cast<f32x4 *>(&merged[wave][4 * LANES]) = f32x4{row.reference, row.most, row.sum, 0.0f};
+        }
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            const f32x4 s = *reinterpret_cast<const f32x4 *>(&merged[w][4 * LANES]), y = *reinterpret_cast<const f32x4 *>(&merged[w][f]);
+            const float x[4] = {y[0], y[1], y[2], y[3]};
+            row.add(s[0], s[1], s[2], x);
+        }
+        finish(row, first_row);
+    } else {
+        Joined row[kJoinRows / kWaves]; // a wave's rows side by side: their reads are under way together
+#pragma unroll
+        for (int i = 0; i < kJoinRows / kWaves; ++i) gather(row[i], min(first_row + wave + kWaves * i, t.rows - 1), 0, SIDE);
+#pragma unroll
+        for (int i = 0; i < kJoinRows / kWaves; ++i) {
+            across(row[i]);
+            finish(row[i], first_row + wave + kWaves * i);
         }
     }
 }
@@ -836,8 +861,13 @@ template<int T, int D, bool VEC>
 void launch(const CacheForwardArgs &a, const ForwardPlan &plan, hipStream_t stream) {
     const int heads = a.cache.heads;
     const uint32_t large = attention_groups(plan.large, heads), small = attention_groups(plan.small, heads);
-    if (large == 0)
-        hipLaunchKernelGGL((cache_attention_small_kernel<T, D, VEC>), dim3(small), dim3(kThreads), 0, stream, a, plan.small);
+    if (large == 0 && plan.small.waves == 16) {
+        if constexpr (D < 128) // (never asked for otherwise)
+            hipLaunchKernelGGL((cache_attention_small_kernel<T, D, VEC, 16>), dim3(small), dim3(16 * kWave), 0, stream, a, plan.small);
+    } else if (large == 0 && plan.small.waves == 8)
+        hipLaunchKernelGGL((cache_attention_small_kernel<T, D, VEC, 8>), dim3(small), dim3(8 * kWave), 0, stream, a, plan.small);
+    else if (large == 0)
+        hipLaunchKernelGGL((cache_attention_small_kernel<T, D, VEC, kWaves>), dim3(small), dim3(kThreads), 0, stream, a, plan.small);
     else if (a.cache.page_size % kStep == 0)
         hipLaunchKernelGGL((cache_attention_kernel<T, D, VEC, 1>), dim3(large + small), dim3(kThreads), 0, stream, a, plan.large, plan.small,
                 large);
@@ -868,7 +898,7 @@ hipError_t launch_cache_forward(const int width, const CacheForwardArgs &a, cons
     long long groups = 0; // of the kernel, or of the join if that has more
     for (const ForwardPart *part : {&plan.small, &plan.large})
         groups += static_cast<long long>(part->units) * a.cache.heads * std::max(part->chunks, part->chunks > 1 ? part->rows / join_rows(*part) : 1);
-    if (groups >= (1ll << 32) / kThreads) return hipErrorInvalidValue; // threads of a launch
+    if (groups >= (1ll << 32) / (kWave * std::max(kWaves, plan.small.waves))) return hipErrorInvalidValue; // threads of a launch
     const int unit = a.dtype == kFloat32 ? 4 : 8;
     auto fits = [&](const void *p, const rocmkernels_strides &s) {
         return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (s.head % unit) == 0 && (s.token % unit) == 0;

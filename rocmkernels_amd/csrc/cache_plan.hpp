@@ -53,6 +53,7 @@ inline long long page_units(const int tokens, const int batch, const int size) {
 // between `least` and `most` flattened rows; with `direct` every sequence has that many units, otherwise they are searched.
 struct ForwardPart {
     int rows, units, direct, least, most, chunk_steps, chunks;
+    int waves;           // of a workgroup; the waves of a small tile take turns with the steps
     size_t workspace;   // bytes: one partial result for each chunk of each tile
     size_t workspace_at; // where they start
 };
@@ -73,31 +74,43 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
     const long long flat = static_cast<long long>(s.tokens) * group;
     ForwardPlan p{};
     size_t most = 0;
+    // Batches whose sequences have a few rows on average are small work throughout, whatever a single sequence has.
+    const bool small_only = flat <= 16ll * s.batch || flat <= kSmallRows;
+    // `tiles`: about how many of the units have rows, which the division over sequences leaves open.
     // `tiles`: about how many of the units have rows, which the division over sequences leaves open.
     auto cut = [&](ForwardPart &part, const long long tiles, const long long workgroups, const int least_steps) {
         // The keys that a tile may see: all, or its window.
         long long span = max_keys;
         if (radius >= 0) span = std::min(span, (causal ? 1ll : 2ll) * radius + 1 + (part.rows + group - 1) / group + kStep);
         const long long steps = (span + kStep - 1) / kStep;
-        const long long pairs = static_cast<long long>(part.units) * heads;
-        const long long filled = std::max(tiles * heads, 1ll), wanted = std::max((workgroups + filled / 2) / filled, 1ll);
+        const long long pairs = static_cast<long long>(part.units) * heads, filled = std::max(tiles * heads, 1ll);
+        const long long wanted = std::max((workgroups + filled / 2) / filled, 1ll);
         const long long chunks = std::min(wanted, std::max(1ll, steps / least_steps)); // grows with the keys and the window
-        part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks + 3) / 4 * 4; // four waves take turns in a small tile
-        part.chunks = static_cast<int>((steps + part.chunk_steps - 1) / part.chunk_steps);
         const size_t chunk_bytes = static_cast<size_t>(pairs) * part.rows * (width + 4) * sizeof(float);
+        most += chunks > 1 ? chunk_bytes * chunks : 0;
+        part.waves = 4;
+        part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks + 3) / 4 * 4;
+        // Where the chip has room for workgroups of more waves and each of these still has no more than four steps to take, one
+        // chunk for each tile saves the join.
+        if (&part == &p.small && small_only) {
+            for (int waves = width == 128 ? 8 : 16; waves > 4; waves /= 2) {
+                if (steps > 4ll * waves || steps <= waves / 2 || filled * waves > (width == 128 ? 8 : 16) * 256ll) continue;
+                part.waves = waves;
+                part.chunk_steps = static_cast<int>(steps);
+                break;
+            }
+        }
+        part.chunks = static_cast<int>((steps + part.chunk_steps - 1) / part.chunk_steps);
         part.workspace = part.chunks > 1 ? chunk_bytes * part.chunks : 0;
         part.workspace_at = p.workspace;
         p.workspace += part.workspace;
-        most += chunks > 1 ? chunk_bytes * chunks : 0;
     };
-    // Batches whose sequences have a few rows on average are small work throughout, whatever a single sequence has.
-    const bool small_only = flat <= 16ll * s.batch || flat <= kSmallRows;
     if (!small_only) {
         p.large.rows = kLargeTile;
         p.large.units = static_cast<int>(row_units(flat, s.batch, kLargeTile));
         p.large.least = s.batch > 1 ? kSmallRows + 1 : 1;
         p.large.most = 0x7fffffff;
-        cut(p.large, flat / kLargeTile, 512, 8);
+        cut(p.large, flat / kLargeTile, s.batch > 1 ? 256 : 512, 8);
     }
     if (small_only || s.batch > 1) {
         p.small.rows = 16;

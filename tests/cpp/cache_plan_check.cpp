@@ -79,7 +79,7 @@ int main() {
             check(p.small.workspace + p.large.workspace == p.workspace, "parts of the workspace");
             for (const rk::ForwardPart *part : {&p.small, &p.large}) {
                 if (part->units == 0) continue;
-                check(part->rows > 0 && part->rows <= rk::kMaxRows && part->chunks >= 1 && part->chunk_steps >= 1, "part");
+                check(part->waves >= 4 && part->waves <= (width == 128 ? 8 : 16) && part->rows > 0 && part->rows <= rk::kMaxRows && part->chunks >= 1 && part->chunk_steps >= 1, "part");
                 check(part->workspace_at + part->workspace <= p.workspace, "a part lies behind the workspace");
                 if (radius < 0) check(static_cast<long long>(part->chunks) * part->chunk_steps * rk::kStep >= keys, "chunks do not cover the keys");
             }
