@@ -309,17 +309,24 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Few rows a sequence, or a page that a wave holds in registers: a wave for each job.
+bool wave_jobs(const int width, const AppendArgs &a) {
+    return a.seqs.tokens <= 8ll * a.seqs.batch || a.cache.page_size * width <= kWavePage;
+}
+long long job_groups_for(const int width, const AppendArgs &a, const long long jobs) {
+    return wave_jobs(width, a) ? (jobs + kWaves - 1) / kWaves : jobs;
+}
+
 template<int T, int D, bool VEC, int W>
 void launch(const AppendArgs &a, const uint32_t jobs, hipStream_t stream) {
-    const uint32_t job_groups = W > 1 ? jobs : (jobs + kWaves - 1) / kWaves;
+    const uint32_t job_groups = static_cast<uint32_t>(job_groups_for(D, a, jobs));
     const uint32_t query_groups = a.q ? static_cast<uint32_t>((static_cast<int64_t>(a.seqs.tokens) + kWaves - 1) / kWaves) : 0;
     hipLaunchKernelGGL((cache_append_kernel<T, D, VEC, W>), dim3(job_groups + query_groups), dim3(kThreads), 0, stream, a, jobs, job_groups);
 }
 
 template<int T, int D>
 void dispatch(const AppendArgs &a, const bool vec, const uint32_t jobs, hipStream_t stream) {
-    // Few rows a sequence, or a page that a wave holds in registers: a wave for each job.
-    if (a.seqs.tokens <= 8ll * a.seqs.batch || a.cache.page_size * D <= kWavePage) {
+    if (wave_jobs(D, a)) {
         if (vec) launch<T, D, true, 1>(a, jobs, stream);
         else launch<T, D, false, 1>(a, jobs, stream);
     } else {
@@ -345,7 +352,8 @@ hipError_t launch_cache_append(const int width, const AppendArgs &a, hipStream_t
             (!a.cos || (table_fits(a.cos, a.cs) && table_fits(a.sin, a.ss)));
     const int size = a.cache.page_size;
     const long long jobs = page_units(a.seqs.tokens, a.seqs.batch, size) * a.cache.heads * 2;
-    if (jobs + a.seqs.tokens >= (1ll << 32) / kThreads) return hipErrorInvalidValue; // threads of a launch
+    if (jobs >= 0xffffffffll || job_groups_for(width, a, jobs) + a.seqs.tokens / kWaves >= (1ll << 32) / kThreads - 1)
+        return hipErrorInvalidValue; // threads of a launch
     const uint32_t n = static_cast<uint32_t>(jobs);
     if (a.dtype == kFloat32) dispatch<kFloat32>(width, a, vec, n, stream);
     else if (a.dtype == kFloat16) dispatch<kFloat16>(width, a, vec, n, stream);

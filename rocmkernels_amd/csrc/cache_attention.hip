@@ -563,10 +563,14 @@ __device__ __forceinline__ void large_tile(const CacheForwardArgs &a, const Forw
             }
         }
     };
+    // Whether every row of the tile sees every key of a step.
+    auto no_key_hidden = [&](const int key0, const uint32_t absent) __attribute__((always_inline)) {
+        return key0 >= tile_low && key0 + kStep <= tile_high && absent == 0;
+    };
     auto stage = [&](const int index, const uint32_t absent) __attribute__((always_inline)) {
         uint8_t *const k = staged[index & 1], *const v = k + K_BYTES;
         const int key0 = kStep * (step_begin + index);
-        const bool full = key0 >= tile_low && key0 + kStep <= tile_high && absent == 0; // no key that any row does not see
+        const bool full = no_key_hidden(key0, absent);
         uint32_t nans = 0;
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
@@ -626,6 +630,8 @@ __device__ __forceinline__ void large_tile(const CacheForwardArgs &a, const Forw
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sc[b / 2][8 * (b % 2) + j] = (visible >> (8 * (j >> 2) + (j & 3))) & 1u ? sc[b / 2][8 * (b % 2) + j] : -INFINITY;
             }
+        }
+        if (!no_key_hidden(key0, e.absent)) { // staged without its NaN, also for the waves that see every key
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) any_nan |= nan_flags[index & 1][w] != 0;
         }

@@ -88,18 +88,20 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         const long long chunks = std::min(wanted, std::max(1ll, steps / least_steps)); // grows with the keys and the window
         const size_t chunk_bytes = static_cast<size_t>(pairs) * part.rows * (width + 4) * sizeof(float);
         most += chunks > 1 ? chunk_bytes * chunks : 0;
+        bool single = false;
         part.waves = 4;
-        part.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks + 3) / 4 * 4;
-        // Where the chip has room for workgroups of more waves and each of these still has no more than four steps to take, one
-        // chunk for each tile saves the join.
         if (&part == &p.small && small_only) {
+            // More waves a workgroup where the chip has room for them and one chunk then holds the keys in four steps a wave: that saves
+            // the join (16 x 5 drafted rows x 4001 keys, 64-wide: 19.5 -> 14.2 us; 8 waves for several chunks of 1 x 32768: no change).
+            const long long room = (width == 128 ? 8 : 16) * 256ll; // waves at the kernels' registers
             for (int waves = width == 128 ? 8 : 16; waves > 4; waves /= 2) {
-                if (steps > 4ll * waves || steps <= waves / 2 || filled * waves > (width == 128 ? 8 : 16) * 256ll) continue;
+                if (steps > 4ll * waves || steps <= waves / 2 || filled * waves > room) continue;
                 part.waves = waves;
-                part.chunk_steps = static_cast<int>(steps);
+                single = true;
                 break;
             }
         }
+        part.chunk_steps = static_cast<int>(single ? steps : ((steps + chunks - 1) / chunks + 3) / 4 * 4); // whole turns of four waves
         part.chunks = static_cast<int>((steps + part.chunk_steps - 1) / part.chunk_steps);
         part.workspace = part.chunks > 1 ? chunk_bytes * part.chunks : 0;
         part.workspace_at = p.workspace;

@@ -118,6 +118,7 @@ def attention(pages, q, table, starts, lengths, causal=True, radius=-1, max_keys
     tol = np.zeros((tokens, query_heads, width))
     lse, lse_tol = np.full((tokens, query_heads, 2), np.nan), np.zeros((tokens, query_heads, 2))
     weight_step = 2.0 ** -22 if two else 2.0 ** -11
+    exponents = np.clip(((pages.scales.view(np.uint32) >> 23) & 255).astype(int) - 127, LOW, HIGH)
     most = table.shape[1] * size
     if max_keys:
         most = min(most, max_keys)
@@ -128,8 +129,7 @@ def attention(pages, q, table, starts, lengths, causal=True, radius=-1, max_keys
         real = (ids >= 0) & (ids < pages.pages)
         safe = np.where(real, ids, 0)
         for h in range(heads):
-            ek = np.array([exponent_of(s) for s in pages.scales[:, h, 0]])[safe]
-            ev = np.array([exponent_of(s) for s in pages.scales[:, h, 1]])[safe]
+            ek, ev = exponents[safe, h, 0], exponents[safe, h, 1]
             k8, v8 = from_e4m3(pages.k[safe, h, place % size]), from_e4m3(pages.v[safe, h, place % size])
             k, v = k8 * np.exp2(ek.astype(float))[:, None], v8 * np.exp2(ev.astype(float))[:, None]
             for i in range(count):

@@ -1,6 +1,8 @@
 """The paged 8-bit cache on an MI355X: appending against the definition byte by byte, attention against 64 bits within the error
 that its roundings can make (tests/cache_reference.py), and the two together as a decoding program runs them."""
+import ctypes
 import math
+import os
 
 import numpy as np
 import pytest
@@ -375,6 +377,59 @@ def test_attention_hidden_keys_may_hold_anything(device, dtype, width):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [1, 2])
+def test_attention_nan_values_reach_the_rows_that_see_them(device, dtype, group):
+    """Prompts of more than one row tile: for a key among the new rows, some waves of a tile see every key of a step and others do
+    not; each row that sees the NaN has it, also rows of later tiles, for which no key of that step is hidden."""
+    for width, size in ((32, 16), (64, 64), (128, 64)):
+        heads, count, length = 2, 200, 230
+        cache = filled_cache(device, 12 if size > 16 else 20, size, heads, width, 71)
+        table, starts, ends = batch_of(device, [count], [length], size, cache.pages, 8)
+        host, vb = table.cpu().numpy(), cache.values.view(torch.uint8)
+        for position, head, feature in ((3, 0, 1), (35, 1, 2), (100, 0, width - 1), (140, 1, 7), (229, 0, 9)):
+            page, slot = int(host[0, position // size]), position % size
+            vb[page, head, slot // 16, feature, slot % 16] = 0xff
+        q = noise(3, count, heads * group, width).to(DTYPES[dtype]).to(device)
+        check_attention(cache, q, table, starts, ends, f"width {width}")
+        check_attention(cache, q, table, starts, ends, f"width {width} window", radius=50)
+
+
+@pytest.mark.parametrize("batch", [65, 300, 5000])
+def test_many_sequences(device, batch):
+    """More sequences than a round of the search tests, some without rows, some with a few."""
+    r = np.random.RandomState(batch)
+    counts = r.choice([0, 1, 1, 1, 2], batch)
+    if batch == 300:
+        counts[::37] = 40  # prompts among them
+    lengths = counts + r.randint(0, 40, batch)
+    size, heads, width = 16, 1, 32
+    pages = int(((lengths + size - 1) // size).sum()) + 2
+    cache = filled_cache(device, pages, size, heads, width, 72)
+    table, starts, ends = batch_of(device, list(counts), list(lengths), size, pages, 9)
+    tokens = int(counts.sum()) + 3
+    k, v, q = (noise(i, tokens, heads, width).to(torch.float16).to(device) for i in range(3))
+    cos, sin = (t.to(device) for t in tables(100, width))
+    check_append(cache, k, v, table, starts, ends, q, cos, sin, f"batch {batch}")
+    check_attention(cache, q, table, starts, ends, f"batch {batch}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width,size", [(128, 64), (64, 48), (32, 16)])
+def test_mixed_batch(device, dtype, width, size):
+    """A chunk of a prompt, single tokens and drafts over long and short contexts in one call: large and small tiles, each cut into
+    chunks."""
+    counts, lengths = [1, 150, 0, 1, 4, 70, 1], [2500, 2600, 100, 1, 40, 70, 900]
+    heads, group = 2, 4
+    pages = sum((n + size - 1) // size for n in lengths) + 1
+    cache = filled_cache(device, pages, size, heads, width, 73)
+    table, starts, ends = batch_of(device, counts, lengths, size, pages, 9)
+    q = noise(3, sum(counts) + 1, heads * group, width).to(DTYPES[dtype]).to(device)
+    assert kv.workspace(cache, q, table).numel() > 0
+    check_attention(cache, q, table, starts, ends, "mixed")
+    check_attention(cache, q, table, starts, ends, "mixed window", radius=700)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_nan_and_infinite_queries_stay_in_their_row(device, dtype):
     cache = filled_cache(device, 8, 64, 2, 64, 47)
     table, starts, ends = batch_of(device, [4], [140], 64, 8, 8)
@@ -537,6 +592,40 @@ def test_results_repeat_bit_for_bit(device):
     for _ in range(5):
         again = kv.attention(cache, q, table, starts, ends)
         assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
+def test_cpp_wrappers_match_c_entry_points(device):
+    path = os.path.join(os.path.dirname(abi.library_path()), "librocmkernels_cache_gpu_check.so")
+    if not os.path.exists(path):
+        pytest.fail(f"{path} is missing: build it with __graft_entry__.build() (CMake)")
+    abi.lib()
+    S, P, I = abi.Strides, ctypes.c_void_p, ctypes.c_int
+    step = ctypes.CDLL(path).cache_step
+    step.argtypes = [P] * 8 + [abi.Cache, abi.Sequences, I, I, I, I, I] + [S] * 6 + [ctypes.c_ubyte, P, ctypes.c_ulonglong, P]
+    step.restype = ctypes.c_longlong
+    heads, width, size, tokens = 2, 64, 32, 45
+    table, starts, ends = batch_of(device, [1, 44], [3000, 50], size, 120, 3)
+    flat = noise(1, tokens, 8, width).to(torch.bfloat16).to(device)  # q, k and v in one tensor: strides that differ from packed ones
+    q, k, v = flat[:, :4], flat[:, 4:6], flat[:, 6:]
+    cos, sin = (t.to(device) for t in tables(3000, width + 8))
+    cos = cos[:, :width]
+    sin = sin.contiguous()[:, 4:4 + width]
+    caches = [filled_cache(device, 120, size, heads, width, 5) for _ in range(2)]
+    want_q = kv.append(caches[0], k, v, table, starts, ends, q=q, cos=cos, sin=sin)
+    want, want_lse = kv.attention(caches[0], want_q, table, starts, ends, radius=2500)
+    out_q, output, lse = torch.empty_like(want_q), torch.empty_like(want), torch.empty_like(want_lse)
+    workspace = kv.workspace(caches[1], q, table)
+    s = lambda t: S(0, t.stride(1) if t.dim() == 3 else 0, t.stride(0))  # noqa: E731
+    sequences = abi.Sequences(starts.data_ptr(), ends.data_ptr(), table.data_ptr(), 2, tokens, table.shape[1], table.stride(0))
+    need = step(k.data_ptr(), v.data_ptr(), q.data_ptr(), cos.data_ptr(), sin.data_ptr(), out_q.data_ptr(), output.data_ptr(), lse.data_ptr(),
+                caches[1]._struct, sequences, 4, 3000, 0, 2500, 1, s(k), s(v), s(q), s(out_q), s(cos), s(sin), abi.DTYPE_BFLOAT16,
+                workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream)
+    assert need == workspace.numel() > 0
+    torch.cuda.synchronize()
+    assert torch.equal(out_q, want_q) and torch.equal(output, want) and torch.equal(lse, want_lse)
+    for name in ("keys", "values"):
+        assert torch.equal(getattr(caches[0], name).view(torch.uint8), getattr(caches[1], name).view(torch.uint8))
+    assert torch.equal(caches[0].scales, caches[1].scales)
 
 
 def test_no_rows(device):
