@@ -8,7 +8,7 @@
 //     x = hi + lo, 22 bits and more.
 //   * The V scale is part of the softmax reference instead of a product per value: w = 2^(s + ev - M), with M the running maximum
 //     of s + ev over the row, weighs v8 directly and stays in fp16's range whatever the scales are; the sum of 2^s is kept as
-//     sum w 2^-ev in the same units, so O = acc / l. Weights are held 2^7 higher (w <= 2^7 at the reference): they keep all
+//     l = sum w 2^-ev in the same units, so O = acc / l. Weights are held 2^7 higher (w <= 2^7 at the reference): they keep all
 //     11 bits down to 2^-21 of it. The reference moves only when a score passes it by more than 2^8 (w <= 2^15).
 //   * S^T = K Q^T and O^T = V^T P^T: a lane holds the scores of one query row (column lane % 16), so the softmax needs no
 //     exchange but the maximum over the four lanes of a column. A wave takes 64 keys a step, as 4 tiles of 16. Row r of tile t is
@@ -31,6 +31,10 @@ namespace {
 
 constexpr float kWeightShift = 7.0f;   // weights are 2^7 at the reference
 constexpr float kLazyRange = 8.0f;     // and reach 2^15 before it moves
+// Sums of weights are held 2^12 lower: with a scale of 2^-100 (V all zero) 2^25 weights of 2^15 then add up within FP32's range, and
+// with one of 2^120 a weight of 2^7 is still no less than 2^-125.
+constexpr float kSumShift = 12.0f;
+constexpr float kSumScale = 0x1p-12f;
 
 __device__ __forceinline__ f32x4 mfma_16(const f16x8 a, const f16x8 b, const f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -104,7 +108,7 @@ template<int T, bool VEC, int N>
 __device__ __forceinline__ void finish_row(const CacheForwardArgs &a, const int64_t token, const int head, const int feature,
         const float (&acc)[N], const float l, const float reference, const float m, const bool writes_lse) {
     const bool nan_row = isnan(l), has_keys = l > 0.0f;
-    const float factor = has_keys ? 1.0f / l : (nan_row ? NAN : 0.0f);
+    const float factor = has_keys ? kSumScale / l : (nan_row ? NAN : 0.0f);
     float o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = has_keys ? acc[i] * factor : factor;
@@ -112,7 +116,7 @@ __device__ __forceinline__ void finish_row(const CacheForwardArgs &a, const int6
     if (writes_lse && a.lse) {
         float *const p = a.lse + 2 * (token * a.query_heads + head);
         p[0] = has_keys ? m / kLog2e : (nan_row ? NAN : -INFINITY);
-        p[1] = has_keys ? l * exp2_fast(reference - m - kWeightShift) : (nan_row ? NAN : 0.0f);
+        p[1] = has_keys ? l * exp2_fast(reference - m - kWeightShift + kSumShift) : (nan_row ? NAN : 0.0f);
     }
 }
 
@@ -337,7 +341,7 @@ __device__ __forceinline__ void small_tile(const CacheForwardArgs &a, const Forw
             for (int j = 0; j < 8; ++j) sum += w[j];
             split_terms<TWO>(wh[u], wl[u], w);
         }
-        l = fmaf(sum, inverse, l);
+        l = fmaf(sum * kSumScale, inverse, l);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll
@@ -676,7 +680,7 @@ __device__ __forceinline__ void large_tile(const CacheForwardArgs &a, const Forw
             for (int j = 0; j < 8; ++j) sum += w[j];
             split_terms<TWO>(wh, wl, w);
             if (b % BLOCKS == BLOCKS - 1) {
-                l = fmaf(sum, power(-static_cast<int8_t>(e.exps[of] >> 8)), l);
+                l = fmaf(sum * kSumScale, power(-static_cast<int8_t>(e.exps[of] >> 8)), l);
                 sum = 0.0f;
             }
 #pragma unroll

@@ -81,6 +81,20 @@ int main() {
                 if (part->units == 0) continue;
                 check(part->waves >= 4 && part->waves <= (width == 128 ? 8 : 16) && part->rows > 0 && part->rows <= rk::kMaxRows && part->chunks >= 1 && part->chunk_steps >= 1, "part");
                 check(part->workspace_at + part->workspace <= p.workspace, "a part lies behind the workspace");
+                // The steps of any tile fit the chunks: rows of neighbouring tokens anywhere, against their window.
+                for (int trial = 0; trial < 5; ++trial) {
+                    const bool causal = round % 2 == 0;
+                    const int row0 = pick(0, 300), rows = pick(1, part->rows), position = pick(-100, keys);
+                    const int from = position + row0 / group, to = position + (row0 + rows - 1) / group;
+                    long long low = 0, high = keys;
+                    if (radius >= 0) {
+                        low = std::max(0, from - radius);
+                        high = std::min<long long>(high, static_cast<long long>(to) + radius + 1);
+                    }
+                    if (causal) high = std::min<long long>(high, to + 1);
+                    const long long steps = high > low ? (high + rk::kStep - 1) / rk::kStep - low / rk::kStep : 0;
+                    check(steps <= static_cast<long long>(part->chunks) * part->chunk_steps, "a tile has more steps than its chunks");
+                }
                 if (radius < 0) check(static_cast<long long>(part->chunks) * part->chunk_steps * rk::kStep >= keys, "chunks do not cover the keys");
             }
             // Every number of rows belongs to exactly one part, and a part with one unit a sequence holds all its rows.

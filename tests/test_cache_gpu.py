@@ -339,6 +339,24 @@ def test_attention_zero_keys_and_tiny_queries(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_over_many_keys_of_no_value(device, dtype, rows):
+    """V all zero (the smallest scale there is) over 65536 keys whose scores rise by just less than what moves the reference: sums of
+    weights over 2^-100 stay in range, and lse is exact."""
+    size, length, width = 128, 65536, 32
+    cache = kv.KVCache.empty(length // size, size, 1, width, device)
+    cache.scales[..., 0] = 1.0
+    position = torch.arange(length, device=device)
+    low = (position % 1024 < 256).view(-1, 1, size // 16, 16)
+    cache.keys.view(torch.uint8).view(-1, 1, size // 16, 16, width)[..., 0] = torch.where(low, 0xb8, 0).to(torch.uint8)  # -1 or 0
+    table = torch.arange(length // size, dtype=torch.int32, device=device)[None]
+    starts, ends = (torch.tensor(t, dtype=torch.int32, device=device) for t in ([0, rows], [length]))
+    q = torch.zeros((rows, 1, width), dtype=DTYPES[dtype], device=device)
+    q[..., 0] = 30.5  # scores of 0 and -30.5 / sqrt(32) = -5.39, that is -7.78 in the exponent of 2
+    check_attention(cache, q, table, starts, ends, causal=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("width", [32, 64])
 def test_attention_hidden_keys_may_hold_anything(device, dtype, width):
     """NaN in K, V and their scales where a row does not look: behind the end, in front of the window, behind its own position."""
