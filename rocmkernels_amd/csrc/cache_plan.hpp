@@ -121,7 +121,7 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         p.small.units = small_only ? static_cast<int>(row_units(flat, s.batch, 16)) : s.batch * p.small.direct;
         p.small.least = 1;
         p.small.most = small_only ? 0x7fffffff : kSmallRows;
-        // 64 sequences of up to 8192 keys, 8 heads: 512 workgroups 132 us, 1024 137, 2048 133, 3072 138. Beside large tiles, which hold half
+        // 64 sequences of up to 8192 keys, 8 heads: 512 workgroups 132 us, 1024 137, 2048 133. Beside large tiles, which hold half
         // the chip for longer, few chunks: 512 84 us, 1024 86, 2048 90 (32 sequences of up to 4096 keys, one with 512 new rows).
         cut(p.small, small_only ? std::max(flat / 16, static_cast<long long>(std::min(s.batch, s.tokens))) : s.batch, small_only ? 2048 : 512, 16);
     }
