@@ -68,6 +68,33 @@ struct ForwardPlan {
 constexpr int kSmallRows = 32;  // sequences of up to this many flattened rows are small work where both kinds may be
 constexpr int kLargeTile = 128; // rows of a large tile
 
+// How many workgroups the large tiles are to make, and the waves of one: four, or two teams of four that take turns with a tile's steps
+// and merge in LDS, which needs no join but gives a compute unit to one tile. `filled` tiles of all heads together, about; `steps`
+// of the keys that a tile may see. Fewer of them never mean more workspace: where they change the waves, the smaller number makes fewer
+// chunks.
+// us with four waves, then with two teams; fp16 and bf16 32 heads on 8, 128-wide, but where a width is given:
+//   one sequence, 768 rows x 4096 keys 91, 73; 1024 x 4096 94, 77; 300 x 32768 268, 199; 64-wide 1500 x 1500 31.6, 25.0; but 1536 x 4096
+//     (384 tiles) 118, 118; 64 x 2000 (16 tiles) 35, 37
+//   several, 256 x 2048 twice to four times 54, 44; 128 x 3000 six times 76, 60; 64-wide FP32 2 x 1500 x 1500 (281 tiles) 49, 47, ragged
+//     4 x 1500 50, 55
+//   one prompt beside 31 tokens, 384 x 2048 53, 43; 512 x 4096 84, 80; but 512 x 8192 136, 167; 256 x 4096 (64 tiles) 62, 79; 1024
+//     x 4096 beside 63 (264 tiles) 136, 172: the tokens' streams then wait for the tiles
+// Where several sequences have many keys, the longest one's steps in a row count: three chunks a tile (ragged 4 x 256 x 8192 145 -> 107,
+// 8 x 128 x 8192 186 -> 109, 64-wide FP32 2 x 1500 x 6000 179 -> 152, ragged 148 -> 107).
+inline int large_waves(const int batch, const long long flat, const long long filled, const long long steps, long long &workgroups) {
+    const bool prompts = batch == 1 || flat >= static_cast<long long>(kLargeTile) * batch; // not: mostly single tokens
+    // Beside the tokens of a mixed batch, with four waves: 128 workgroups take 108 us, 256 90, 384 90, 512 106.
+    workgroups = batch > 1 ? 256 : 512;
+    if (steps < 8 || filled <= (batch > 1 ? 85 : 64)) return 4;
+    if (batch > 1 && prompts && steps >= 90 && filled < 512) {
+        workgroups = 3 * filled;
+        return 4;
+    }
+    if (filled > (prompts ? 256 : 128) || (!prompts && steps >= 80)) return 4;
+    workgroups = prompts ? 256 / filled * filled : filled;
+    return 8;
+}
+
 inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, const int heads, const int query_heads, const int max_keys,
         const int radius, const bool causal) {
     const int group = query_heads / heads;
@@ -76,27 +103,31 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
     size_t most = 0;
     // Batches whose sequences have a few rows on average are small work throughout, whatever a single sequence has.
     const bool small_only = flat <= 16ll * s.batch || flat <= kSmallRows;
-    // `tiles`: about how many of the units have rows, which the division over sequences leaves open.
+    // The steps of the keys that a tile of `rows` rows may see: all, or its window.
+    auto span_steps = [&](const int rows) {
+        long long span = max_keys;
+        if (radius >= 0) span = std::min(span, (causal ? 1ll : 2ll) * radius + 1 + (rows + group - 1) / group + kStep);
+        return (span + kStep - 1) / kStep;
+    };
+    long long large_groups = 0;
+    const int waves = small_only ? 4 : large_waves(s.batch, flat, std::max(flat / kLargeTile, 1ll) * heads, span_steps(kLargeTile), large_groups);
     // `tiles`: about how many of the units have rows, which the division over sequences leaves open.
     auto cut = [&](ForwardPart &part, const long long tiles, const long long workgroups, const int least_steps) {
-        // The keys that a tile may see: all, or its window.
-        long long span = max_keys;
-        if (radius >= 0) span = std::min(span, (causal ? 1ll : 2ll) * radius + 1 + (part.rows + group - 1) / group + kStep);
-        const long long steps = (span + kStep - 1) / kStep;
+        const long long steps = span_steps(part.rows);
         const long long pairs = static_cast<long long>(part.units) * heads, filled = std::max(tiles * heads, 1ll);
         const long long wanted = std::max((workgroups + filled / 2) / filled, 1ll);
         const long long chunks = std::min(wanted, std::max(1ll, steps / least_steps)); // grows with the keys and the window
         const size_t chunk_bytes = static_cast<size_t>(pairs) * part.rows * (width + 4) * sizeof(float);
         most += chunks > 1 ? chunk_bytes * chunks : 0;
         bool single = false;
-        part.waves = 4;
+        part.waves = waves;
         if (&part == &p.small && small_only) {
             // More waves a workgroup where the chip has room for them and one chunk then holds the keys in four steps a wave: that saves
             // the join (16 x 5 drafted rows x 4001 keys, 64-wide: 19.5 -> 14.2 us; 8 waves for several chunks of 1 x 32768: no change).
             const long long room = (width == 128 ? 8 : 16) * 256ll; // waves at the kernels' registers
-            for (int waves = width == 128 ? 8 : 16; waves > 4; waves /= 2) {
-                if (steps > 4ll * waves || steps <= waves / 2 || filled * waves > room) continue;
-                part.waves = waves;
+            for (int more = width == 128 ? 8 : 16; more > 4; more /= 2) {
+                if (steps > 4ll * more || steps <= more / 2 || filled * more > room) continue;
+                part.waves = more;
                 single = true;
                 break;
             }
@@ -112,8 +143,7 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         p.large.units = static_cast<int>(row_units(flat, s.batch, kLargeTile));
         p.large.least = s.batch > 1 ? kSmallRows + 1 : 1;
         p.large.most = 0x7fffffff;
-        // In the same mixed batch 128 workgroups take 108 us, 256 90, 384 90, 512 106: the small tiles fill the other half of the chip.
-        cut(p.large, flat / kLargeTile, s.batch > 1 ? 256 : 512, 8);
+        cut(p.large, flat / kLargeTile, large_groups, waves == 8 ? 16 : 8);
     }
     if (small_only || s.batch > 1) {
         p.small.rows = 16;
@@ -123,7 +153,7 @@ inline ForwardPlan plan_cache_forward(const int width, const SequenceView &s, co
         p.small.most = small_only ? 0x7fffffff : kSmallRows;
         // 64 sequences of up to 8192 keys, 8 heads: 512 workgroups 132 us, 1024 137, 2048 133. Beside large tiles, which hold half
         // the chip for longer, few chunks: 512 84 us, 1024 86, 2048 90 (32 sequences of up to 4096 keys, one with 512 new rows).
-        cut(p.small, small_only ? std::max(flat / 16, static_cast<long long>(std::min(s.batch, s.tokens))) : s.batch, small_only ? 2048 : 512, 16);
+        cut(p.small, small_only ? std::max(flat / 16, static_cast<long long>(std::min(s.batch, s.tokens))) : s.batch, small_only ? 2048 : 2048 / waves, 16);
     }
     p.workspace_most = most;
     return p;

@@ -111,6 +111,14 @@ int main() {
             }
         }
     }
+    // Large tiles of eight waves, as tests/test_cache_gpu.py expects them: batch, tokens, heads, group, keys, radius, waves.
+    for (const auto &c : {std::vector<int>{1, 131, 13, 5, 704, -1, 8}, {1, 131, 13, 5, 704, 500, 8}, {1, 131, 13, 5, 2240, -1, 8},
+                 {4, 251, 13, 5, 704, -1, 8}, {11, 161, 16, 5, 912, -1, 8}, {1, 130, 13, 5, 1008, -1, 8}, {1, 130, 13, 5, 1008, 100, 4},
+                 {1, 20, 13, 5, 1008, -1, 4}}) {
+        const rk::SequenceView s{nullptr, nullptr, nullptr, c[0], c[1], 1, 1};
+        const rk::ForwardPlan p = rk::plan_cache_forward(64, s, c[2], c[2] * c[3], c[4], c[5], true);
+        check(p.large.waves == c[6] && (p.small.units == 0 || p.small.waves == c[6]), "waves of a large tile");
+    }
     std::printf("%d failure(s)\n", failures);
     return failures != 0;
 }

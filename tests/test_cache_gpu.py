@@ -447,6 +447,58 @@ def test_mixed_batch(device, dtype, width, size):
     check_attention(cache, q, table, starts, ends, "mixed window", radius=700)
 
 
+# Batches whose large tiles two teams of waves share (tests/cpp/cache_plan_check.cpp holds the plan to it): heads, group, counts,
+# lengths, masks. One prompt in one chunk of an odd and an even number of steps, and in two chunks; prompts beside each other, one of
+# them short and one without rows; a prompt beside single tokens.
+TEAMS = [
+    (13, 5, [130], [681], [{"radius": 500}, {"causal": False, "radius": 260}]),
+    (13, 5, [130], [2200], [{}]),
+    (13, 5, [100, 60, 0, 90], [700, 60, 30, 513], [{}]),
+    (16, 5, [150] + [1] * 10, [900, 1, 64, 65, 300, 512, 513, 577, 640, 899, 20], [{}, {"radius": 520}]),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width,size", [(32, 64), (64, 48), (128, 16)])
+def test_attention_by_two_teams(device, dtype, width, size):
+    for n, (heads, group, counts, lengths, masks) in enumerate(TEAMS):
+        pages = sum((m + size - 1) // size for m in lengths) + 1
+        cache = filled_cache(device, pages, size, heads, width, 81 + n)
+        table, starts, ends = batch_of(device, counts, lengths, size, pages, 10 + n)
+        q = noise(4 + n, sum(counts) + 1, heads * group, width).to(DTYPES[dtype]).to(device)
+        for how in masks:
+            check_attention(cache, q, table, starts, ends, f"{counts} {lengths} {how}", **how)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width,size", [(32, 32), (64, 64), (128, 64)])
+def test_attention_by_two_teams_at_the_edges(device, dtype, width, size):
+    """Sequences far shorter than the table allows (no step for one team, or for both), rows without keys, pages that are not there,
+    and NaN in V at positions of either team's steps; twice the same bits."""
+    heads, group, count = 13, 5, 130
+    pages = (1000 + size - 1) // size + 1
+    q = noise(4, count, heads * group, width).to(DTYPES[dtype]).to(device)
+    for length in (0, 1, 64, 100, 129):
+        cache = filled_cache(device, pages, size, heads, width, 91)
+        table, starts, ends = batch_of(device, [count], [1000], size, pages, 11)
+        ends[:] = length
+        check_attention(cache, q, table, starts, ends, f"length {length}", causal=True)
+        check_attention(cache, q, table, starts, ends, f"length {length}, all", causal=False)
+    cache = filled_cache(device, pages, size, heads, width, 92)
+    table, starts, ends = batch_of(device, [count], [1000], size, pages, 12)
+    host, vb = table.cpu().numpy().copy(), cache.values.view(torch.uint8)
+    for position, head, feature in ((3, 0, 1), (70, 1, 2), (140, 3, width - 1), (880, 4, 7), (930, 5, 0), (999, 12, 9)):
+        vb[int(host[0, position // size]), head, position % size // 16, feature, position % 16] = 0x7f
+    check_attention(cache, q, table, starts, ends, "NaN in V")
+    check_attention(cache, q, table, starts, ends, "NaN in V, window", radius=500)
+    table[0, 1] = -1
+    table[0, 400 // size] = pages
+    table[0, 999 // size] = -7
+    check_attention(cache, q, table, starts, ends, "pages that are not there")
+    first, second = (kv.attention(cache, q, table, starts, ends) for _ in range(2))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(first, second))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_nan_and_infinite_queries_stay_in_their_row(device, dtype):
     cache = filled_cache(device, 8, 64, 2, 64, 47)
